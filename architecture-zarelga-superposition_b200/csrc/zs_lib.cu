@@ -10,4 +10,6 @@
 #include "zs_adam.cu"
 #include "zs_comm.cu"
 #include "zs_sparse.cu"
+#include "zs_paged.cu"
+#include "zs_paged_attn.cu"
 #include "zs_api.cu"

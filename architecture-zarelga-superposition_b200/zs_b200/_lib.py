@@ -26,6 +26,13 @@ class AdamWTensor(ctypes.Structure):
                 ("inv_bc2_host", _f32), ("shadow_bf16", _vp), ("n", _i64)]
 
 
+class KvCache(ctypes.Structure):
+    """zs_kv_cache (include/zs.h)."""
+    _fields_ = [("kv", _vp), ("block_table", _vp), ("seq_lens", _vp), ("ref_count", _vp), ("num_pages", _i64),
+                ("n_layers", _i32), ("n_kv_heads", _i32), ("page_size", _i32), ("head_dim", _i32), ("max_seqs", _i32),
+                ("max_pages", _i32)]
+
+
 # name -> (restype, argtypes); mirrors include/zs.h
 _SIGNATURES = {
     "zs_version": (_i32, []),
@@ -111,6 +118,19 @@ _SIGNATURES = {
     "zs_xent_backward_workspace": (_sz, [_i64, _i64, _i32]),
     "zs_xent_backward": (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp,
                                 _i64, _vp, _sz, _i32, _vp]),
+    "zs_paged_append": (_i32, [_vp, _i64, _vp, _vp, _f32, _vp, _vp, _i64, _i64, _i32, _vp, _vp, _i64, _i64, _vp, _i64,
+                               _i32, _vp, _vp, _i32, _i64, _i32, _i32, _i32, _i32, _vp, _i32, _vp]),
+    "zs_paged_prompt_attention": (_i32, [_vp, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i32, _vp, _vp, _i32, _i64, _i32,
+                                         _i32, _i32, _i32, _i32, _f32, _vp, _i32, _vp, _i64, _vp, _vp, _i32, _vp]),
+    "zs_paged_decode_workspace": (_sz, [_i32, _i32, _i32, _i32]),
+    "zs_paged_decode_attention": (_i32, [_vp, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i32, _vp, _i32, _i32, _i32, _i32,
+                                         _i32, _i32, _f32, _vp, _i32, _vp, _i64, _vp, _vp, _i32, _vp, _sz, _vp]),
+    "zs_kv_workspace": (_sz, [ctypes.POINTER(KvCache), _i64]),
+    "zs_kv_extend": (_i32, [ctypes.POINTER(KvCache), _vp, _vp, _i64, _vp, _sz, _vp]),
+    "zs_kv_fork": (_i32, [ctypes.POINTER(KvCache), _vp, _vp, _i64, _vp, _sz, _vp]),
+    "zs_kv_free": (_i32, [ctypes.POINTER(KvCache), _vp, _i64, _vp]),
+    "zs_kv_compact": (_i32, [ctypes.POINTER(KvCache), _vp, _sz, _vp]),
+    "zs_kv_copy_pages": (_i32, [ctypes.POINTER(KvCache), _vp, _vp, _i64, _vp, _sz, _vp]),
 }
 
 

@@ -52,6 +52,7 @@ extern "C" {
 #define ZS_DEVERR_TIMEOUT_DRAIN 0x08
 #define ZS_DEVERR_INDEX 0x10       /* an index input was out of range; the element was skipped */
 #define ZS_DEVERR_TIMEOUT_PEER 0x20 /* a wait for a peer GPU's flag expired (zs_ce_allreduce) */
+#define ZS_DEVERR_CACHE_FULL 0x40  /* a cache had no free page or a slot no room; the request was refused */
 
 /* dtype codes */
 #define ZS_F32 0
@@ -654,6 +655,111 @@ int zs_sparse_rmsprop_step(float* param, int64_t num_rows, int64_t d, int64_t ld
                            long long* step_counter, const int64_t* rows, const float* values, int64_t ld_values,
                            int64_t n, const float* lr_ptr, float lr, double beta, float eps, int unit_norm,
                            void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------ paged key-value cache
+ *
+ * Serving a trained model (no counterpart in the reference, whose inference.py
+ * :25-73 runs the whole sequence again for every token).  A layer's keys and
+ * values lie in pages:
+ *   k_pages, v_pages [num_pages, Hkv, page, hd], the last three dimensions
+ *   packed, page_stride elements between pages; page 16, 32, 64 or 128 tokens,
+ *   hd 64 or 128, bf16 or f16, 16-byte aligned.
+ *   block_table int32 [num_seqs, max_pages], rows of bt_ld: a sequence's pages
+ *   in order.  seq_lens int32 [num_seqs]: tokens in the cache, this call's new
+ *   ones included.  cu_seqlens int32 [num_seqs + 1]: sequence s's new tokens are
+ *   the packed rows cu_seqlens[s] .. cu_seqlens[s + 1) and lie at its positions
+ *   seq_lens[s] - n_s .. seq_lens[s]).  A packed row outside every sequence or
+ *   at a negative position is padding.
+ * A page id out of range records ZS_DEVERR_INDEX: nothing is stored there, and
+ * it reads as zeros.  So does a length beyond the table: the attention cuts it
+ * to the table, the append stores nothing beyond.
+ *
+ * zs_paged_append: per head, zero-centred RMSNorm (q_weight / k_weight f32 [hd],
+ *   gain 1 + w; both NULL: none) and rotation of the first `rot` pairs
+ *   (i, i + hd / 2) by cos/sin f32 [table_rows, rot] (rows of table_ld) at the
+ *   token's position, in f32, rounded once.  qkv: packed rows of ld elements
+ *   (H query heads, Hkv key heads, Hkv value heads, anything after); q_out
+ *   [tokens, H, hd]; keys and values go to their pages.  cu_seqlens NULL: row s
+ *   is sequence s's one new token (tokens == num_seqs).  Padding: q_out is zero,
+ *   nothing is stored.
+ * zs_paged_prompt_attention: o[t, h] = sum_k softmax_k(scale q[t, h] . K_k) V_k
+ *   over the keys k <= p of row t's sequence (p its position; p - k < window when
+ *   window > 0), key head h / (H / Hkv); k_sink [H, hd] (nullable): one more
+ *   logit scale q . k_sink whose value is zero; gate (nullable, q's dtype, rows
+ *   of ldg): o is multiplied by sigmoid(gate[t, h]).  lse (nullable) f32
+ *   [tokens, H]: the log-sum-exp, sink included.  Padding and rows that see no
+ *   key: o is zero (lse of padding outside every sequence: -inf).  A NaN or
+ *   infinity in a value of the sequence may reach every row of the same
+ *   sequence; what lies in the pages outside the sequence reaches none.
+ * zs_paged_decode_attention: the same for one token per sequence (row s), with
+ *   the keys of a sequence split over blocks and joined in a fixed order;
+ *   seq_lens[s] == 0 marks an empty slot (o zero).  The workspace holds partial
+ *   results of this call only; calls that may overlap need one each.
+ */
+int zs_paged_append(const void* qkv, int64_t ld, const float* q_weight, const float* k_weight, float eps,
+                    const float* cos, const float* sin, int64_t table_ld, int64_t table_rows, int rot, void* k_pages,
+                    void* v_pages, int64_t page_stride, int64_t num_pages, const int* block_table, int64_t bt_ld,
+                    int max_pages, const int* seq_lens, const int* cu_seqlens, int num_seqs, int64_t tokens, int H,
+                    int Hkv, int hd, int page, void* q_out, int dtype, void* stream);
+int zs_paged_prompt_attention(const void* q, int64_t ldq, const void* k_pages, const void* v_pages,
+                              int64_t page_stride, int64_t num_pages, const int* block_table, int64_t bt_ld,
+                              int max_pages, const int* seq_lens, const int* cu_seqlens, int num_seqs, int64_t tokens,
+                              int H, int Hkv, int hd, int page, int window, float scale, const void* k_sink,
+                              int sink_dtype, const void* gate, int64_t ldg, void* o, float* lse, int dtype,
+                              void* stream);
+size_t zs_paged_decode_workspace(int num_seqs, int H, int Hkv, int hd);
+int zs_paged_decode_attention(const void* q, int64_t ldq, const void* k_pages, const void* v_pages,
+                              int64_t page_stride, int64_t num_pages, const int* block_table, int64_t bt_ld,
+                              int max_pages, const int* seq_lens, int num_seqs, int H, int Hkv, int hd, int page,
+                              int window, float scale, const void* k_sink, int sink_dtype, const void* gate,
+                              int64_t ldg, void* o, float* lse, int dtype, void* workspace, size_t workspace_bytes,
+                              void* stream);
+
+/*
+ * The cache's bookkeeping, on the device: kv [n_layers, 2, num_pages,
+ * n_kv_heads, page_size, head_dim] 16-bit elements (keys, then values, of each
+ * layer), block_table [max_seqs, max_pages] (-1: no page), seq_lens [max_seqs],
+ * ref_count [num_pages] (the rows that hold the page; 0: free).  Requests are
+ * served in order and take the lowest-numbered free pages, so the tables after
+ * a call are a function of the tables before it.  num_pages <= 2000000.  A slot
+ * or page out of range, or a target named again by a later request, records
+ * ZS_DEVERR_INDEX; a request without room records ZS_DEVERR_CACHE_FULL, and so
+ * does every later request of the call that needs a page; refused requests
+ * change nothing.
+ *   zs_kv_extend: slots[i] grows by tokens[i] >= 0 tokens, with pages for them.
+ *   zs_kv_fork: dst[i] becomes a copy of src[i] as it was before the call (what
+ *     dst[i] held is let go; src[i] == dst[i] stays): whole pages are shared, the
+ *     rows of a last partial page are copied into a free page.
+ *   zs_kv_free: slots become empty; pages that no row holds are free.
+ *   zs_kv_compact: the pages in use become pages 0 .. U-1: the k-th free page
+ *     below U takes the k-th used page from U on.
+ *   zs_kv_copy_pages: dst[i] = src[i], every layer's keys and values.  A dst that
+ *     is also a src is refused.
+ * Workspace: zs_kv_workspace(cache, n) bytes (n = 0 for zs_kv_compact).
+ */
+typedef struct {
+  void* kv;
+  int* block_table;
+  int* seq_lens;
+  int* ref_count;
+  int64_t num_pages;
+  int n_layers;
+  int n_kv_heads;
+  int page_size;
+  int head_dim;
+  int max_seqs;
+  int max_pages;
+} zs_kv_cache;
+
+size_t zs_kv_workspace(const zs_kv_cache* cache, int64_t n);
+int zs_kv_extend(const zs_kv_cache* cache, const int* slots, const int* tokens, int64_t n, void* workspace,
+                 size_t workspace_bytes, void* stream);
+int zs_kv_fork(const zs_kv_cache* cache, const int* src, const int* dst, int64_t n, void* workspace,
+               size_t workspace_bytes, void* stream);
+int zs_kv_free(const zs_kv_cache* cache, const int* slots, int64_t n, void* stream);
+int zs_kv_compact(const zs_kv_cache* cache, void* workspace, size_t workspace_bytes, void* stream);
+int zs_kv_copy_pages(const zs_kv_cache* cache, const int* src, const int* dst, int64_t n, void* workspace,
+                     size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
