@@ -8,6 +8,8 @@
 // logit or -inf.
 #include "zs_common.cuh"
 
+#include <type_traits>
+
 namespace zs {
 namespace paged {
 
@@ -127,6 +129,488 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const AttnArgs a) {
   }
 }
 
+// ------------------------------------------------------------------------ decode
+//
+// One token per sequence: the cache is read once and hardly anything is computed, so the
+// kernel is bound by HBM.  The work is the list of 64-key tiles of every (sequence, key head,
+// block of 16 query heads), in that order, cut into equal runs, one per block: a batch of
+// sequences of any lengths loads every SM alike.  A block walks its run, and whatever part of
+// a (sequence, head) ends in it is finished there; parts of one that several blocks share go
+// to the workspace (at most two per block, the run's first and last) and
+// paged_join_kernel adds them in the order of the blocks.
+//
+// Warp 4 loads the pages of a tile with TMA (128-byte swizzle) into a ring of stages; warps
+// 0-3 each take 16 of its keys: S = Q K^T and O += P V by mma.sync with the group's query heads
+// as the 16 rows, P straight from the accumulators of S, and a running (max, sum, O) of their
+// own, joined through shared memory when a part ends.  mma.sync, not tcgen05: a 128-row tile
+// would hold 1 to 16 rows of work, and the products are a tenth of the time of the loads.
+
+constexpr int DEC_TILE = 64;              // keys per tile
+constexpr int DEC_MAX_BLOCKS = 320;       // two per SM
+constexpr int DEC_ROWS = 16;              // query heads per block of rows
+constexpr int DEC_LDO = 40;               // floats per row of the join buffer (32 + padding against bank conflicts)
+
+template <int HD>
+struct DecSmem {
+  static constexpr int STAGES = HD == 128 ? 3 : 6;
+  static constexpr int MAT = DEC_TILE * HD * 2;                 // K or V of one tile
+  static constexpr int STAGE = 2 * MAT;
+  static constexpr int OFF_O = STAGES * STAGE;                  // [4 warps][16 rows][32 columns] f32, padded rows
+  static constexpr int OFF_ML = OFF_O + 4 * DEC_ROWS * DEC_LDO * 4;  // max and sum [2][4][16]
+  static constexpr int OFF_BAR = OFF_ML + 2 * 4 * DEC_ROWS * 4;
+  static constexpr int OFF_MISC = OFF_BAR + 2 * STAGES * 8;
+  static constexpr int TOTAL = OFF_MISC + 64;
+  static constexpr int ALLOC = TOTAL + 1024;
+};
+
+// Partial results: [block][2][16 rows][HD + 2] (O, max, sum), then the running tile counts.
+__host__ __device__ constexpr int64_t part_floats(int hd) { return (int64_t)DEC_ROWS * (hd + 2); }
+
+struct Span {              // the key tiles of a sequence
+  int len, first_key, first_tile, tiles;
+};
+__device__ __forceinline__ Span span_of(const AttnArgs& a, int seq) {
+  Span s;
+  const int len = cut_length(a, seq);
+  s.len = len > 0 ? len : 0;
+  s.first_key = a.window > 0 && s.len > a.window ? s.len - a.window : 0;
+  s.first_tile = s.first_key / DEC_TILE;
+  // an empty sequence has one tile with no key in it, so that its rows are written
+  s.tiles = max((s.len + DEC_TILE - 1) / DEC_TILE - s.first_tile, 1);
+  return s;
+}
+
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Barrier of the four product warps; whether any thread's flag was set, the same answer for all.
+__device__ __forceinline__ bool consumer_any(bool flag) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "bar.red.or.pred q, 1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)flag)
+      : "memory");
+  return r != 0;
+}
+
+// 3-D tiled TMA load: c0 in elements, c1 row inside the page, c2 page.
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
+      "[%2];" ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+
+// The sink's logit of query head h (log2 units), summed over the 8 lanes that call together.
+template <typename T, int HD>
+__device__ __forceinline__ float sink_logit8(const AttnArgs& a, int64_t tok, int h) {
+  const int part = threadIdx.x & 7;
+  const T* q = reinterpret_cast<const T*>(a.q) + tok * a.ldq + (int64_t)h * HD;
+  float dot = 0.f;
+#pragma unroll
+  for (int e = 0; e < HD / 8; ++e) {
+    const int c = part * (HD / 8) + e;
+    dot = fmaf(to_f32(q[c]), load_any(a.k_sink, a.sink_dtype, (int64_t)h * HD + c), dot);
+  }
+#pragma unroll
+  for (int off = 4; off > 0; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
+  return dot * a.scale_log2;
+}
+
+// Four columns of a finished row: the sink joined, the sum divided out, the gate applied.
+template <typename T, int HD>
+__device__ __forceinline__ void finish_row(const AttnArgs& a, int64_t tok, int h, int col, float m, float l,
+                                           const float (&o)[4], float z, bool write_lse) {
+  float f = 1.f;
+  if (a.k_sink != nullptr) {
+    const float mt = fmaxf(m, z);
+    f = m == -INFINITY ? 0.f : exp2f(m - mt);
+    l = l * f + exp2f(z - mt);
+    m = mt;
+  }
+  float inv = l > 0.f ? f / l : (l != l ? l : 0.f);
+  if (a.gate != nullptr) inv *= 1.f / (1.f + expf(-to_f32(reinterpret_cast<const T*>(a.gate)[tok * a.ldg + h])));
+  const typename Pair<T>::type v[2] = {Pair<T>::from_f(o[0] * inv, o[1] * inv), Pair<T>::from_f(o[2] * inv, o[3] * inv)};
+  *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.o) + (tok * a.H + h) * HD + col) =
+      make_uint2(*reinterpret_cast<const uint32_t*>(&v[0]), *reinterpret_cast<const uint32_t*>(&v[1]));
+  if (write_lse && a.lse != nullptr) a.lse[tok * a.H + h] = l > 0.f ? (m + log2f(l)) * 0.6931471805599453f : (l != l ? l : -INFINITY);
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(160, 2)
+    paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                        const AttnArgs a, float* parts, int64_t* counts) {
+  using L = DecSmem<HD>;
+  constexpr int ATOMS = HD / 64;
+  constexpr int KS = HD / 16;              // k-steps of S
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
+  uint64_t* empty = full + L::STAGES;
+  int64_t* s_run = reinterpret_cast<int64_t*>(smem + L::OFF_MISC);   // tiles in all, then tiles before s_seq
+  int* s_seq = reinterpret_cast<int*>(smem + L::OFF_MISC + 16);
+  volatile int* s_abort = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 20);
+  int64_t* s_warp = reinterpret_cast<int64_t*>(smem + L::OFF_O);     // scratch of the count below
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int G = a.H / a.Hkv;
+  const int blocks_g = (G + DEC_ROWS - 1) / DEC_ROWS;
+  const int units = a.Hkv * blocks_g;      // per sequence
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < L::STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 4);
+    }
+    *s_abort = 0;
+    fence_barrier_init();
+  }
+  // Count the tiles: thread t those of a contiguous share of the sequences.
+  const int per = (a.num_seqs + 159) / 160;
+  const int q0 = min(a.num_seqs, (int)threadIdx.x * per), q1 = min(a.num_seqs, q0 + per);
+  int64_t mine = 0;
+  for (int s = q0; s < q1; ++s) mine += span_of(a, s).tiles;
+  int64_t inc = mine;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int64_t o = __shfl_up_sync(0xffffffffu, inc, off);
+    if (lane >= off) inc += o;
+  }
+  if (lane == 31) s_warp[warp] = inc;
+  __syncthreads();
+  int64_t before = inc - mine, total = 0;
+  for (int w = 0; w < 5; ++w) {
+    if (w < warp) before += s_warp[w];
+    total += s_warp[w];
+  }
+  const int64_t all = total * units;
+  const int64_t nb = min((int64_t)gridDim.x, all);      // blocks with work
+  const int64_t begin = blockIdx.x * all / nb, end = (blockIdx.x + 1) * all / nb;
+  const bool works = blockIdx.x < nb;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the join waits for this grid's end itself
+  {
+    int64_t at = before;
+    for (int s = q0; s < q1; ++s) {
+      const int n = span_of(a, s).tiles;
+      if (blockIdx.x == 0) counts[s] = at;
+      if (works && begin >= at * units && begin < (at + n) * units) {
+        *s_seq = s;
+        s_run[1] = at;
+      }
+      at += n;
+    }
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) counts[a.num_seqs] = total;
+  __syncthreads();
+  if (!works) return;
+
+  int seq = *s_seq;
+  Span sp = span_of(a, seq);
+  int unit, tile;
+  {
+    const int64_t rest = begin - s_run[1] * units;
+    unit = (int)(rest / sp.tiles);
+    tile = (int)(rest - (int64_t)unit * sp.tiles);
+  }
+  auto advance = [&]() {
+    if (++tile < sp.tiles) return;
+    tile = 0;
+    if (++unit < units) return;
+    unit = 0;
+    ++seq;
+    if (seq < a.num_seqs) sp = span_of(a, seq);
+  };
+
+  if (warp == 4) {
+    // ---------------------------------------------------------------- loads
+    const int rows = min(a.page, DEC_TILE);            // rows per box
+    const int per_tile = DEC_TILE / rows;              // pages of a tile
+    const int boxes = per_tile * ATOMS * 2;            // lane = (page, atom, K or V)
+    const int pg = lane / (2 * ATOMS), at = (lane >> 1) % ATOMS, kv = lane & 1;
+    int it = 0;
+    uint32_t issued = 0, par = 0;
+    for (int64_t g = begin; g < end; ++g, ++it) {
+      const int st = it % L::STAGES;
+      const int hk = unit / blocks_g;
+      const int key = (sp.first_tile + tile) * DEC_TILE + pg * rows;
+      int page = (int)a.num_pages;                     // past the pool: TMA fills zeros
+      if (lane < boxes && key < sp.len && key + rows > sp.first_key) {
+        page = __ldg(a.block_table + seq * a.bt_ld + key / a.page);
+        if ((unsigned)page >= (unsigned)a.num_pages) {
+          record_error(ZS_DEVERR_INDEX);
+          page = (int)a.num_pages;
+        }
+      }
+      if (!warp_wait(&empty[st], ((it / L::STAGES) & 1) ^ 1, s_abort, ZS_DEVERR_TIMEOUT_PRODUCER)) break;
+      if (lane == 0) mbar_arrive_expect_tx(&full[st], L::STAGE);
+      __syncwarp();
+      if (lane < boxes)
+        tma_load_3d(smem + st * L::STAGE + kv * L::MAT + at * (DEC_TILE * 128) + pg * rows * 128, kv ? &tmV : &tmK,
+                    &full[st], at * 64, hk * a.page + key % a.page, page);
+      issued |= 1u << st;
+      par = (par & ~(1u << st)) | ((uint32_t)((it / L::STAGES) & 1) << st);
+      advance();
+    }
+    for (int s = 0; s < L::STAGES; ++s)                // copies in flight land before the warp leaves
+      if (issued >> s & 1) mbar_wait(&full[s], par >> s & 1, nullptr, ZS_DEVERR_TIMEOUT_DRAIN);
+    return;
+  }
+
+  // ------------------------------------------------------------------ products
+  const int r4 = lane >> 2, c4 = lane & 3;
+  float* s_o = reinterpret_cast<float*>(smem + L::OFF_O);
+  float* s_m = reinterpret_cast<float*>(smem + L::OFF_ML);
+  float* s_l = s_m + 4 * DEC_ROWS;
+  uint32_t qf[KS][4];
+  float o[HD / 8][4];
+  float m[2], l[2];
+  int it = 0, first = 1;                               // first: the part began with the block's run
+  int64_t g = begin;
+  while (g < end) {
+    // a part: tiles [tile, ...) of (seq, unit), to the unit's or the run's end
+    const int hk = unit / blocks_g, g0 = (unit - hk * blocks_g) * DEC_ROWS;
+    const int h0 = hk * G + g0, nrow = min(DEC_ROWS, G - g0);
+    const bool from_start = tile == 0;
+    const int64_t left = end - g;
+    const int n = (int)min((int64_t)(sp.tiles - tile), left);
+    const bool to_end = tile + n == sp.tiles;
+    const int pseq = seq;
+    {
+      const T* q = reinterpret_cast<const T*>(a.q) + (int64_t)seq * a.ldq + (int64_t)h0 * HD + c4 * 2;
+#pragma unroll
+      for (int kk = 0; kk < KS; ++kk)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int row = r4 + (x & 1) * 8;
+          qf[kk][x] = row < nrow ? *reinterpret_cast<const uint32_t*>(q + row * HD + kk * 16 + (x >> 1) * 8) : 0u;
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < HD / 8; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[c][e] = 0.f;
+    m[0] = m[1] = -INFINITY;
+    l[0] = l[1] = 0.f;
+    for (int j = 0; j < n; ++j, ++it) {
+      const int st = it % L::STAGES;
+      const int key0 = (sp.first_tile + tile + j) * DEC_TILE + warp * 16;
+      if (!warp_wait(&full[st], (it / L::STAGES) & 1, s_abort, ZS_DEVERR_TIMEOUT_EPILOGUE)) break;
+      const uint32_t kb = smem_u32(smem + st * L::STAGE), vb = kb + L::MAT;
+      float s[2][4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[0][e] = s[1][e] = 0.f;
+      const int krow = warp * 16 + (lane >> 4) * 8 + (lane & 7);
+#pragma unroll
+      for (int kk = 0; kk < KS; ++kk) {
+        const int ch = kk * 2 + ((lane >> 3) & 1);     // 16-byte chunk of the row
+        uint32_t b[4];
+        ldsm_x4(kb + (ch >> 3) * (DEC_TILE * 128) + krow * 128 + (((ch & 7) ^ (krow & 7)) << 4), b);
+        mma_16816<T>(s[0], qf[kk], b[0], b[1]);
+        mma_16816<T>(s[1], qf[kk], b[2], b[3]);
+      }
+      const bool edge = key0 + 16 > sp.len || key0 < sp.first_key;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[t][e] *= a.scale_log2;
+          if (edge) {
+            const int k = key0 + t * 8 + c4 * 2 + (e & 1);
+            if (k >= sp.len || k < sp.first_key) s[t][e] = -INFINITY;
+          }
+        }
+      // running maximum, raised only when it grows by more than 2^8 (P and the sums stay far from
+      // the range's end, and O is rescaled rarely)
+      float f[2];
+      bool grow = false;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float mx = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        f[r] = 1.f;
+        if (mx > m[r] + 8.f) {
+          f[r] = m[r] == -INFINITY ? 0.f : exp2f(m[r] - mx);
+          m[r] = mx;
+          l[r] *= f[r];
+          grow = true;
+        }
+      }
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int c = 0; c < HD / 8; ++c) {
+          o[c][0] *= f[0];
+          o[c][1] *= f[0];
+          o[c][2] *= f[1];
+          o[c][3] *= f[1];
+        }
+      }
+      // P in the cache's type for the second product, its sum in f32 before the rounding
+      uint32_t p[4];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float mu = m[r] == -INFINITY ? 0.f : m[r];
+          const float e0 = attn::fast_exp2(s[t][2 * r] - mu), e1 = attn::fast_exp2(s[t][2 * r + 1] - mu);
+          l[r] += e0 + e1;
+          const typename Pair<T>::type pp = Pair<T>::from_f(e0, e1);
+          p[t * 2 + r] = *reinterpret_cast<const uint32_t*>(&pp);
+        }
+      const int vrow = warp * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
+      uint32_t keep[2] = {0xffffffffu, 0xffffffffu};   // values of keys that are not seen count as zero
+      if (edge) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int k = key0 + t * 8 + c4 * 2;
+          keep[t] = (k < sp.len && k >= sp.first_key ? 0xffffu : 0u) |
+                    (k + 1 < sp.len && k + 1 >= sp.first_key ? 0xffff0000u : 0u);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < HD / 8; c += 2) {
+        const int ch = c + (lane >> 4);
+        uint32_t b[4];
+        ldsm_x4_t(vb + (ch >> 3) * (DEC_TILE * 128) + vrow * 128 + (((ch & 7) ^ (vrow & 7)) << 4), b);
+        if (edge) {
+          b[0] &= keep[0];
+          b[1] &= keep[1];
+          b[2] &= keep[0];
+          b[3] &= keep[1];
+        }
+        mma_16816<T>(o[c], p, b[0], b[1]);
+        mma_16816<T>(o[c + 1], p, b[2], b[3]);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[st]);
+    }
+    // ------------------------------------------------------------- the part's end
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+      if (c4 == 0) {
+        s_m[warp * DEC_ROWS + r4 + r * 8] = m[r];
+        s_l[warp * DEC_ROWS + r4 + r * 8] = l[r];
+      }
+    }
+    const bool whole = from_start && to_end;
+    const int row = threadIdx.x >> 3, col = (threadIdx.x & 7) * 4;
+    const int h = h0 + min(row, nrow - 1);
+    const float z = whole && a.k_sink != nullptr ? sink_logit8<T, HD>(a, pseq, h) : 0.f;
+    float* part = parts + ((int64_t)blockIdx.x * 2 + (first ? 0 : 1)) * part_floats(HD) + row * (HD + 2);
+    bool stop = false;
+#pragma unroll
+    for (int ps = 0; ps < HD / 32; ++ps) {             // 32 columns at a time
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float* dst = s_o + (warp * DEC_ROWS + r4) * DEC_LDO + c * 8 + c4 * 2;
+        *reinterpret_cast<float2*>(dst) = make_float2(o[ps * 4 + c][0], o[ps * 4 + c][1]);
+        *reinterpret_cast<float2*>(dst + 8 * DEC_LDO) = make_float2(o[ps * 4 + c][2], o[ps * 4 + c][3]);
+      }
+      consumer_any(false);
+      float mt = -INFINITY, lt = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) mt = fmaxf(mt, s_m[w * DEC_ROWS + row]);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float mw = s_m[w * DEC_ROWS + row];
+        const float fw = mw == -INFINITY ? 0.f : exp2f(mw - mt);
+        lt = fmaf(fw, s_l[w * DEC_ROWS + row], lt);
+        const float4 x = *reinterpret_cast<const float4*>(s_o + (w * DEC_ROWS + row) * DEC_LDO + col);
+        acc[0] = fmaf(fw, x.x, acc[0]);
+        acc[1] = fmaf(fw, x.y, acc[1]);
+        acc[2] = fmaf(fw, x.z, acc[2]);
+        acc[3] = fmaf(fw, x.w, acc[3]);
+      }
+      if (row < nrow) {
+        if (whole) {
+          finish_row<T, HD>(a, pseq, h, ps * 32 + col, mt, lt, acc, z, ps == 0 && col == 0);
+        } else {
+          float2* dst = reinterpret_cast<float2*>(part + ps * 32 + col);
+          dst[0] = make_float2(acc[0], acc[1]);
+          dst[1] = make_float2(acc[2], acc[3]);
+          if (ps == 0 && col == 0) *reinterpret_cast<float2*>(part + HD) = make_float2(mt, lt);
+        }
+      }
+      stop = consumer_any(*s_abort);                   // also: the buffer may be written again
+    }
+    if (stop) return;
+    g += n;
+    tile += n - 1;
+    advance();
+    first = 0;
+  }
+}
+
+// Block (sequence, unit): the sum of its parts, where more than one block of the decode
+// kernel had a part of it.
+template <typename T, int HD>
+__global__ void __launch_bounds__(128) paged_join_kernel(const AttnArgs a, const float* parts, const int64_t* counts,
+                                                         int decode_blocks) {
+  const int G = a.H / a.Hkv;
+  const int blocks_g = (G + DEC_ROWS - 1) / DEC_ROWS;
+  const int units = a.Hkv * blocks_g;
+  const int seq = blockIdx.x, unit = blockIdx.y;
+  const int hk = unit / blocks_g, g0 = (unit - hk * blocks_g) * DEC_ROWS;
+  const int h0 = hk * G + g0, nrow = min(DEC_ROWS, G - g0);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int64_t all = counts[a.num_seqs] * units, nb = min((int64_t)decode_blocks, all);
+  const int64_t tiles = counts[seq + 1] - counts[seq];
+  const int64_t t0 = counts[seq] * units + unit * tiles, t1 = t0 + tiles - 1;
+  // block of tile t: the last b with floor(b * all / nb) <= t
+  const int64_t b0 = ((t0 + 1) * nb - 1) / all, b1 = ((t1 + 1) * nb - 1) / all;
+  if (b0 == b1) return;
+  const int row = threadIdx.x >> 3;
+  const int h = h0 + min(row, nrow - 1);
+  const float z = a.k_sink != nullptr ? sink_logit8<T, HD>(a, seq, h) : 0.f;
+  if (row >= nrow) return;
+  auto part_of = [&](int64_t b) {
+    // a block's first part lies in its slot 0; one that starts inside the block's run in slot 1
+    return parts + (b * 2 + (b * all / nb < t0 ? 1 : 0)) * part_floats(HD) + row * (HD + 2);
+  };
+  float mt = -INFINITY;
+  for (int64_t b = b0; b <= b1; ++b) mt = fmaxf(mt, part_of(b)[HD]);
+#pragma unroll
+  for (int ps = 0; ps < HD / 32; ++ps) {
+    const int col = ps * 32 + (threadIdx.x & 7) * 4;
+    float lt = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int64_t b = b0; b <= b1; ++b) {
+      const float* part = part_of(b);
+      const float mw = part[HD], fw = mw == -INFINITY ? 0.f : exp2f(mw - mt);
+      lt = fmaf(fw, part[HD + 1], lt);
+      const float2 x = *reinterpret_cast<const float2*>(part + col), y = *reinterpret_cast<const float2*>(part + col + 2);
+      acc[0] = fmaf(fw, x.x, acc[0]);
+      acc[1] = fmaf(fw, x.y, acc[1]);
+      acc[2] = fmaf(fw, y.x, acc[2]);
+      acc[3] = fmaf(fw, y.y, acc[3]);
+    }
+    finish_row<T, HD>(a, seq, h, col, mt, lt, acc, z, col == 0);
+  }
+}
+
 }  // namespace paged
 }  // namespace zs
 
@@ -185,9 +669,65 @@ static int launch_plain(const paged::AttnArgs& a, int hd, int dtype, cudaStream_
   return ZS_OK;
 }
 
+static int make_page_tmap(CUtensorMap* m, const void* base, int dtype, int hd, int64_t rows, int64_t pages,
+                          int64_t page_stride, int box_rows) {
+  auto fn = encode_fn();
+  if (fn == nullptr) return ZS_ERR_CUDA;
+  cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)rows, (cuuint64_t)pages};
+  cuuint64_t strides[2] = {(cuuint64_t)hd * 2, (cuuint64_t)page_stride * 2};
+  cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1};
+  cuuint32_t es[3] = {1, 1, 1};
+  const CUresult r = fn(m, dtype == ZS_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                        const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    zs_last_cuda_error_ref() = 100000 + (int)r;
+    return ZS_ERR_CUDA;
+  }
+  return ZS_OK;
+}
+
+template <typename T, int HD>
+static int launch_decode(const paged::AttnArgs& a, int dtype, void* workspace, cudaStream_t stream) {
+  using L = paged::DecSmem<HD>;
+  CUtensorMap tk, tv;
+  const int box = a.page < paged::DEC_TILE ? a.page : paged::DEC_TILE;
+  int rc = make_page_tmap(&tk, a.k_pages, dtype, HD, (int64_t)a.Hkv * a.page, a.num_pages, a.page_stride, box);
+  if (rc != ZS_OK) return rc;
+  rc = make_page_tmap(&tv, a.v_pages, dtype, HD, (int64_t)a.Hkv * a.page, a.num_pages, a.page_stride, box);
+  if (rc != ZS_OK) return rc;
+  // no more blocks than tiles that the table (or the window) leaves room for
+  const int G = a.H / a.Hkv, units = a.Hkv * ((G + paged::DEC_ROWS - 1) / paged::DEC_ROWS);
+  int64_t most = ((int64_t)a.max_pages * a.page + paged::DEC_TILE - 1) / paged::DEC_TILE;
+  if (a.window > 0) most = min(most, (int64_t)(a.window + paged::DEC_TILE - 2) / paged::DEC_TILE + 1);
+  const int64_t all = most * a.num_seqs * units;
+  const int resident = 2 * num_sms() < paged::DEC_MAX_BLOCKS ? 2 * num_sms() : paged::DEC_MAX_BLOCKS;
+  const int blocks = (int)(all < resident ? all : resident);
+  int64_t* counts = reinterpret_cast<int64_t*>((reinterpret_cast<uintptr_t>(workspace) + 15) & ~uintptr_t(15));
+  float* parts = reinterpret_cast<float*>(counts + ((a.num_seqs + 2) & ~1));
+  ZS_CUDA_TRY(cudaFuncSetAttribute(paged::paged_decode_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::ALLOC));
+  paged::paged_decode_kernel<T, HD><<<blocks, 160, L::ALLOC, stream>>>(tk, tv, a, parts, counts);
+  ZS_CUDA_TRY(cudaGetLastError());
+  if (most == 1) return ZS_OK;                         // nothing can be split
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)a.num_seqs, (unsigned)units);
+  cfg.blockDim = dim3(128);
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  ZS_CUDA_TRY(cudaLaunchKernelEx(&cfg, paged::paged_join_kernel<T, HD>, a, (const float*)parts,
+                                 (const int64_t*)counts, blocks));
+  return ZS_OK;
+}
+
 extern "C" size_t zs_paged_decode_workspace(int num_seqs, int H, int Hkv, int hd) {
-  (void)num_seqs, (void)H, (void)Hkv, (void)hd;
-  return 16;
+  (void)H, (void)Hkv;
+  if (num_seqs < 0 || hd < 0) return 0;
+  return (size_t)((num_seqs + 4) * 8 + paged::DEC_MAX_BLOCKS * 2 * paged::part_floats(hd) * 4 + 64);
 }
 
 extern "C" int zs_paged_decode_attention(const void* q, int64_t ldq, const void* k_pages, const void* v_pages,
@@ -204,7 +744,11 @@ extern "C" int zs_paged_decode_attention(const void* q, int64_t ldq, const void*
   if (rc != ZS_OK) return rc;
   ZS_REQUIRE(workspace && workspace_bytes >= zs_paged_decode_workspace(num_seqs, H, Hkv, hd), ZS_ERR_WORKSPACE);
   ZS_BIND(q);
-  return launch_plain(a, hd, dtype, stream);
+  if (dtype == ZS_BF16)
+    return hd == 128 ? launch_decode<__nv_bfloat16, 128>(a, dtype, workspace, stream)
+                     : launch_decode<__nv_bfloat16, 64>(a, dtype, workspace, stream);
+  return hd == 128 ? launch_decode<__half, 128>(a, dtype, workspace, stream)
+                   : launch_decode<__half, 64>(a, dtype, workspace, stream);
 }
 
 extern "C" int zs_paged_prompt_attention(const void* q, int64_t ldq, const void* k_pages, const void* v_pages,

@@ -30,55 +30,79 @@ import torch
 from . import _lib as Z
 
 PAGE_SIZES = (16, 32, 64, 128)
-_DTYPES = (torch.bfloat16, torch.float16)
+_DTYPES = {torch.bfloat16: Z.ZS_BF16, torch.float16: Z.ZS_F16}
 
 
-def _refuse(cond, msg):
-    if cond:
-        raise Z.ZsError(msg)
+def _fail(msg):
+    raise Z.ZsError(msg)
 
 
 def _no_grad(*tensors):
-    _refuse(torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors),
-            "the paged operators have no gradient: call them under torch.no_grad() or on detached tensors")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                _fail("the paged operators have no gradient: call them under torch.no_grad() or on detached tensors")
 
 
 def _same_device(first, *tensors):
-    Z.require_cuda(first, *tensors)
+    """Index of the CUDA device that holds all the tensors."""
+    dev = first.get_device()
     for t in tensors:
-        _refuse(t is not None and t.device != first.device,
-                f"all tensors must be on one device (got {first.device} and {t.device if t is not None else None})")
+        if t is not None and t.get_device() != dev:
+            Z.require_cuda(t)
+            _fail(f"all tensors must be on one device (got {first.device} and {t.device})")
+    if dev < 0:
+        Z.require_cuda(first)
+    return dev
 
+
+# One decode step is a few microseconds of kernel time per call, so the checks below read each
+# tensor's shape and strides once and build their messages only when they refuse.
 
 def _pages(k_pages, v_pages):
-    """(num_pages, Hkv, page, hd, page stride) of a layer's pages."""
-    _refuse(k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype,
-            f"k_pages and v_pages must be [num_pages, Hkv, page, hd] of one shape and dtype (got "
-            f"{tuple(k_pages.shape)} {k_pages.dtype}, {tuple(v_pages.shape)} {v_pages.dtype})")
-    P, Hkv, page, hd = k_pages.shape
-    _refuse(k_pages.dtype not in _DTYPES, f"the cache holds bf16 or f16 (got {k_pages.dtype})")
-    _refuse(page not in PAGE_SIZES or hd not in (64, 128) or P < 1 or Hkv < 1,
-            f"pages hold {PAGE_SIZES} tokens of head_dim 64 or 128 (got {tuple(k_pages.shape)})")
-    strides = (page * hd, hd, 1)
-    for t in (k_pages, v_pages):
-        _refuse(t.stride()[1:] != strides or t.stride(0) % 8 or (P > 1 and t.stride(0) < Hkv * page * hd),
-                f"pages must be packed in their last three dimensions (got strides {t.stride()})")
-    _refuse(P > 1 and k_pages.stride(0) != v_pages.stride(0), "k_pages and v_pages must have one page stride")
-    return P, Hkv, page, hd, max(k_pages.stride(0), Hkv * page * hd)
+    """(num_pages, Hkv, page, hd, page stride, dtype) of a layer's pages."""
+    shape, dtype = k_pages.shape, k_pages.dtype
+    if len(shape) != 4 or v_pages.shape != shape or v_pages.dtype != dtype:
+        _fail(f"k_pages and v_pages must be [num_pages, Hkv, page, hd] of one shape and dtype (got "
+              f"{tuple(shape)} {dtype}, {tuple(v_pages.shape)} {v_pages.dtype})")
+    P, Hkv, page, hd = shape
+    if dtype not in _DTYPES or page not in PAGE_SIZES or hd not in (64, 128) or P < 1 or Hkv < 1:
+        _fail(f"the cache holds bf16 or f16 pages of {PAGE_SIZES} tokens of head_dim 64 or 128 (got {dtype} "
+              f"{tuple(shape)})")
+    ks, vs = k_pages.stride(), v_pages.stride()
+    run = page * hd
+    if P == 1:
+        ks, vs = (Hkv * run,) + ks[1:], (Hkv * run,) + vs[1:]
+    if ks != vs or ks[0] % 8 or ks[0] < Hkv * run or ks[3] != 1 or ks[2] != hd or (ks[1] != run and Hkv > 1):
+        _fail("k_pages and v_pages must be packed in their last three dimensions, with one page stride that is a "
+              f"multiple of 8 (got strides {k_pages.stride()}, {v_pages.stride()})")
+    return P, Hkv, page, hd, ks[0], dtype
+
+
+def _int32_list(name, t, want):
+    if t.dtype != torch.int32 or t.shape != (want,) or not t.is_contiguous():
+        _fail(f"{name} must be a contiguous int32 [{want}] (got {t.dtype} {tuple(t.shape)})")
 
 
 def _tables(block_table, seq_lens, cu_seqlens):
-    _refuse(block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.size(1) < 1
-            or (block_table.size(1) > 1 and block_table.stride(1) != 1)
-            or (block_table.size(0) > 1 and block_table.stride(0) < block_table.size(1)),
-            f"block_table must be int32 [num_seqs, max_pages], rows packed (got {block_table.dtype} "
-            f"{tuple(block_table.shape)}, strides {block_table.stride()})")
-    n = block_table.size(0)
-    for name, t, want in (("seq_lens", seq_lens, n), ("cu_seqlens", cu_seqlens, n + 1)):
-        _refuse(t is not None and (t.dim() != 1 or t.dtype != torch.int32 or t.numel() != want or not t.is_contiguous()),
-                f"{name} must be a contiguous int32 [{want}] (got {t.dtype if t is not None else None} "
-                f"{tuple(t.shape) if t is not None else None})")
-    return n, max(block_table.stride(0), block_table.size(1))
+    """(num_seqs, max_pages, row stride) of the block table."""
+    shape = block_table.shape
+    if len(shape) != 2 or block_table.dtype != torch.int32 or shape[1] < 1:
+        _fail(f"block_table must be int32 [num_seqs, max_pages] (got {block_table.dtype} {tuple(shape)})")
+    n, m = shape
+    ld, inner = block_table.stride()
+    if (inner != 1 and m > 1) or (ld < m and n > 1):
+        _fail(f"block_table rows must be packed and apart (got strides {block_table.stride()})")
+    _int32_list("seq_lens", seq_lens, n)
+    if cu_seqlens is not None:
+        _int32_list("cu_seqlens", cu_seqlens, n + 1)
+    return n, m, max(ld, m)
+
+
+def _aligned(t):
+    if t.stride(0) != 1:
+        t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
 
 
 def paged_append(qkvg, k_pages, v_pages, block_table, seq_lens, *, n_heads, cu_seqlens=None, q_weight=None,
@@ -91,90 +115,119 @@ def paged_append(qkvg, k_pages, v_pages, block_table, seq_lens, *, n_heads, cu_s
     by cos/sin f32 [positions, rot] at the token's position (None: no rotation); f32 arithmetic,
     one rounding.  cu_seqlens None: row s is sequence s's one new token.  A row outside every
     sequence, or at a negative position (an empty slot), gets a zero q and stores nothing."""
-    _same_device(k_pages, v_pages, qkvg, block_table, seq_lens, cu_seqlens, q_weight, k_weight, cos, sin)
+    dev = _same_device(k_pages, v_pages, qkvg, block_table, seq_lens, cu_seqlens, q_weight, k_weight, cos, sin)
     _no_grad(qkvg, k_pages, v_pages, q_weight, k_weight)
-    P, Hkv, page, hd, stride = _pages(k_pages, v_pages)
+    P, Hkv, page, hd, stride, dtype = _pages(k_pages, v_pages)
+    n, m, bt_ld = _tables(block_table, seq_lens, cu_seqlens)
     H = int(n_heads)
-    n, bt_ld = _tables(block_table, seq_lens, cu_seqlens)
-    _refuse(qkvg.dim() != 2 or qkvg.dtype != k_pages.dtype or qkvg.size(1) < (H + 2 * Hkv) * hd or H < 1 or H % Hkv,
-            f"qkvg must be {k_pages.dtype} [T, >= (H + 2 Hkv) hd] with H % Hkv == 0 (got {qkvg.dtype} "
-            f"{tuple(qkvg.shape)}, H={H}, Hkv={Hkv}, hd={hd})")
-    T = qkvg.size(0)
-    _refuse(cu_seqlens is None and T != n, f"without cu_seqlens each sequence has one row (got {T} rows, {n} sequences)")
-    _refuse((q_weight is None) != (k_weight is None), "q_weight and k_weight come together")
+    width = (H + 2 * Hkv) * hd
+    shape = qkvg.shape
+    if len(shape) != 2 or qkvg.dtype != dtype or shape[1] < width or H < 1 or H % Hkv:
+        _fail(f"qkvg must be {dtype} [T, >= (H + 2 Hkv) hd] with H % Hkv == 0 (got {qkvg.dtype} {tuple(shape)}, "
+              f"H={H}, Hkv={Hkv}, hd={hd})")
+    T = shape[0]
+    if cu_seqlens is None and T != n:
+        _fail(f"without cu_seqlens each sequence has one row (got {T} rows, {n} sequences)")
+    if (q_weight is None) != (k_weight is None):
+        _fail("q_weight and k_weight come together")
     if q_weight is not None:
         for w in (q_weight, k_weight):
-            _refuse(w.dtype != torch.float32 or w.shape != (hd,), f"norm weights must be f32 [{hd}]")
+            if w.dtype != torch.float32 or w.shape != (hd,):
+                _fail(f"norm weights must be f32 [{hd}] (got {w.dtype} {tuple(w.shape)})")
         q_weight, k_weight = _aligned(q_weight), _aligned(k_weight)
-    _refuse((cos is None) != (sin is None), "cos and sin come together")
-    rot, rows, table_ld = 0, 0, 0
+    if (cos is None) != (sin is None):
+        _fail("cos and sin come together")
+    rot = rows = table_ld = 0
     if cos is not None:
-        for t in (cos, sin):
-            _refuse(t.dim() != 2 or t.dtype != torch.float32 or t.shape != cos.shape or t.size(1) > hd // 2
-                    or t.size(0) < 1, f"cos and sin must be f32 [positions, rot <= {hd // 2}] of one shape")
-        if (cos.stride(1) != 1 or sin.stride(1) != 1 or cos.stride(0) != sin.stride(0)
-                or cos.stride(0) < cos.size(1)):
+        shape = cos.shape
+        if (len(shape) != 2 or sin.shape != shape or cos.dtype != torch.float32 or sin.dtype != torch.float32
+                or shape[1] > hd // 2 or shape[0] < 1):
+            _fail(f"cos and sin must be f32 [positions, rot <= {hd // 2}] of one shape (got {cos.dtype} "
+                  f"{tuple(shape)}, {sin.dtype} {tuple(sin.shape)})")
+        rows, rot = shape
+        st = cos.stride()
+        if sin.stride() != st or st[1] != 1 or st[0] < rot:
             cos, sin = cos.contiguous(), sin.contiguous()
-        rows, rot = cos.shape
-        table_ld = max(cos.stride(0), rot)
-    q = torch.empty(T, H, hd, dtype=qkvg.dtype, device=qkvg.device)
+            st = (rot, 1)
+        table_ld = st[0]
+    q = torch.empty((T, H, hd), dtype=dtype, device=qkvg.device)
     if T == 0 or n == 0:
         return q.zero_()
-    if qkvg.stride(1) != 1 or qkvg.stride(0) % 8 or qkvg.data_ptr() % 16 or (T > 1 and qkvg.stride(0) < qkvg.size(1)):
-        qkvg = qkvg[:, :(H + 2 * Hkv) * hd].contiguous()
-        qkvg = qkvg.clone() if qkvg.data_ptr() % 16 else qkvg
+    ld, inner = qkvg.stride()
+    x = qkvg.data_ptr()
+    if inner != 1 or ld % 8 or x % 16 or (T > 1 and ld < width):
+        qkvg = qkvg[:, :width].clone(memory_format=torch.contiguous_format)
+        x, ld = qkvg.data_ptr(), width
     Z.count(1)
-    Z.check(Z.lib().zs_paged_append(
-        qkvg.data_ptr(), max(qkvg.stride(0), (H + 2 * Hkv) * hd), Z.ptr(q_weight), Z.ptr(k_weight), float(eps),
-        Z.ptr(cos) if rot else None, Z.ptr(sin) if rot else None, table_ld, rows, rot, k_pages.data_ptr(),
-        v_pages.data_ptr(), stride, P, block_table.data_ptr(), bt_ld, block_table.size(1), seq_lens.data_ptr(),
-        Z.ptr(cu_seqlens), n, T, H, Hkv, hd, page, q.data_ptr(), Z.dtype_code(q.dtype), Z.stream_of(q)),
-        "zs_paged_append")
+    rc = Z.lib().zs_paged_append(
+        x, max(ld, width), Z.ptr(q_weight), Z.ptr(k_weight), eps, cos.data_ptr() if rot else None,
+        sin.data_ptr() if rot else None, table_ld, rows, rot, k_pages.data_ptr(), v_pages.data_ptr(), stride, P,
+        block_table.data_ptr(), bt_ld, m, seq_lens.data_ptr(), Z.ptr(cu_seqlens), n, T, H, Hkv, hd, page,
+        q.data_ptr(), _DTYPES[dtype], torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        Z.check(rc, "zs_paged_append")
     return q
 
 
-def _aligned(t):
-    t = t.contiguous()
-    return t.clone() if t.data_ptr() % 16 else t
-
-
-def _attention_inputs(q, k_pages, v_pages, block_table, seq_lens, cu_seqlens, window, k_sink, gate, scale):
-    _same_device(k_pages, v_pages, q, block_table, seq_lens, cu_seqlens, k_sink, gate)
+def _attention(q, k_pages, v_pages, block_table, seq_lens, cu_seqlens, window, k_sink, gate, scale, return_lse, decode):
+    dev = _same_device(k_pages, v_pages, q, block_table, seq_lens, cu_seqlens, k_sink, gate)
     _no_grad(q, k_pages, v_pages, k_sink, gate)
-    P, Hkv, page, hd, stride = _pages(k_pages, v_pages)
-    n, bt_ld = _tables(block_table, seq_lens, cu_seqlens)
-    _refuse(q.dim() != 3 or q.dtype != k_pages.dtype or q.size(2) != hd or q.size(1) < 1 or q.size(1) % Hkv,
-            f"q must be {k_pages.dtype} [T, H, {hd}] with H % Hkv == 0 (got {q.dtype} {tuple(q.shape)}, Hkv={Hkv})")
-    T, H, _ = q.shape
-    _refuse(cu_seqlens is None and T != n, f"q has one row per sequence (got {T} rows, {n} sequences)")
-    w = 0 if window is None else int(window)
-    _refuse(window is not None and (w <= 0 or w >= 1 << 31), f"window must be None or positive (got {window!r})")
+    P, Hkv, page, hd, stride, dtype = _pages(k_pages, v_pages)
+    n, m, bt_ld = _tables(block_table, seq_lens, cu_seqlens)
+    shape = q.shape
+    if len(shape) != 3 or q.dtype != dtype or shape[2] != hd or shape[1] < 1 or shape[1] % Hkv:
+        _fail(f"q must be {dtype} [T, H, {hd}] with H % Hkv == 0 (got {q.dtype} {tuple(shape)}, Hkv={Hkv})")
+    T, H, _ = shape
+    if decode and T != n:
+        _fail(f"q has one row per sequence (got {T} rows, {n} sequences)")
+    w = 0
+    if window is not None:
+        w = int(window)
+        if w <= 0 or w >= 1 << 31:
+            _fail(f"window must be None or positive (got {window!r})")
+    sink_dtype = 0
     if k_sink is not None:
-        _refuse(k_sink.shape != (H, hd), f"k_sink must be [{H}, {hd}] (got {tuple(k_sink.shape)})")
-        k_sink = k_sink.contiguous()
-        Z.dtype_code(k_sink.dtype)
+        if k_sink.shape != (H, hd):
+            _fail(f"k_sink must be [{H}, {hd}] (got {tuple(k_sink.shape)})")
+        if not k_sink.is_contiguous():
+            k_sink = k_sink.contiguous()
+        sink_dtype = Z.dtype_code(k_sink.dtype)
     ldg = 0
     if gate is not None:
-        _refuse(gate.shape != (T, H) or gate.dtype != q.dtype,
-                f"gate must be {q.dtype} [{T}, {H}] (got {gate.dtype} {tuple(gate.shape)})")
-        if (H > 1 and gate.stride(1) != 1) or (T > 1 and gate.stride(0) < H):
+        if gate.shape != (T, H) or gate.dtype != dtype:
+            _fail(f"gate must be {dtype} [{T}, {H}] (got {gate.dtype} {tuple(gate.shape)})")
+        ldg, inner = gate.stride()
+        if (inner != 1 and H > 1) or (ldg < H and T > 1):
             gate = gate.contiguous()
-        ldg = max(gate.stride(0), H)
-    scale = 1.0 / math.sqrt(hd) if scale is None else float(scale)
-    if (q.stride(2) != 1 or (H > 1 and q.stride(1) != hd) or q.stride(0) % 8 or q.data_ptr() % 16
-            or (T > 1 and q.stride(0) < H * hd)):
-        q = q.contiguous()
-        q = q.clone() if q.data_ptr() % 16 else q
-    head = (q.data_ptr(), max(q.stride(0), H * hd), k_pages.data_ptr(), v_pages.data_ptr(), stride, P,
-            block_table.data_ptr(), bt_ld, block_table.size(1), seq_lens.data_ptr())
-    o = torch.empty(T, H, hd, dtype=q.dtype, device=q.device)
-    tail = (H, Hkv, hd, page, w, scale, Z.ptr(k_sink), Z.dtype_code(k_sink.dtype) if k_sink is not None else 0,
-            Z.ptr(gate), ldg, o.data_ptr())
-    return n, head, tail, o, (q, k_sink, gate)
-
-
-def _lse_of(return_lse, o):
-    return torch.empty(o.shape[:2], dtype=torch.float32, device=o.device) if return_lse else None
+            ldg = H
+        ldg = max(ldg, H)
+    o = torch.empty((T, H, hd), dtype=dtype, device=q.device)
+    lse = torch.empty((T, H), dtype=torch.float32, device=q.device) if return_lse else None
+    if T == 0 or n == 0:
+        o.zero_()
+        return (o, lse.fill_(-math.inf)) if return_lse else o
+    ldq, head, inner = q.stride()
+    x = q.data_ptr()
+    if inner != 1 or (head != hd and H > 1) or ldq % 8 or x % 16 or (T > 1 and ldq < H * hd):
+        q = q.clone(memory_format=torch.contiguous_format)
+        x, ldq = q.data_ptr(), H * hd
+    scale = 1.0 / math.sqrt(hd) if scale is None else scale
+    L = Z.lib()
+    args = (x, max(ldq, H * hd), k_pages.data_ptr(), v_pages.data_ptr(), stride, P, block_table.data_ptr(), bt_ld, m,
+            seq_lens.data_ptr())
+    more = (H, Hkv, hd, page, w, scale, Z.ptr(k_sink), sink_dtype, Z.ptr(gate), ldg, o.data_ptr(), Z.ptr(lse),
+            _DTYPES[dtype])
+    stream = torch._C._cuda_getCurrentRawStream(dev)
+    Z.count(1)
+    if decode:
+        size = L.zs_paged_decode_workspace(n, H, Hkv, hd)
+        ws = torch.empty(size, dtype=torch.uint8, device=q.device)
+        rc = L.zs_paged_decode_attention(*args, n, *more, ws.data_ptr(), size, stream)
+    else:
+        rc = L.zs_paged_prompt_attention(*args, cu_seqlens.data_ptr(), n, T, *more, stream)
+    if rc:
+        Z.check(rc, "zs_paged_decode_attention" if decode else "zs_paged_prompt_attention")
+    return (o, lse) if return_lse else o
 
 
 def paged_prompt_attention(q, k_pages, v_pages, block_table, seq_lens, cu_seqlens, *, window=None, k_sink=None,
@@ -185,17 +238,8 @@ def paged_prompt_attention(q, k_pages, v_pages, block_table, seq_lens, cu_seqlen
     k_sink [H, hd]: one more logit q . k_sink per head whose value is zero.  gate [T, H] (q's dtype;
     a strided view will do): o is multiplied by sigmoid(gate).  Rows that see no key, and rows
     outside every sequence, are zero."""
-    n, head, tail, o, keep = _attention_inputs(q, k_pages, v_pages, block_table, seq_lens, cu_seqlens, window, k_sink,
-                                               gate, scale)
-    _refuse(cu_seqlens is None, "cu_seqlens is required")
-    lse = _lse_of(return_lse, o)
-    if o.size(0) == 0 or n == 0:
-        o.zero_()
-        return (o, lse.fill_(-math.inf)) if return_lse else o
-    Z.count(1)
-    Z.check(Z.lib().zs_paged_prompt_attention(*head, cu_seqlens.data_ptr(), n, o.size(0), *tail, Z.ptr(lse),
-                                              Z.dtype_code(o.dtype), Z.stream_of(o)), "zs_paged_prompt_attention")
-    return (o, lse) if return_lse else o
+    return _attention(q, k_pages, v_pages, block_table, seq_lens, cu_seqlens, window, k_sink, gate, scale, return_lse,
+                      False)
 
 
 def paged_decode_attention(q, k_pages, v_pages, block_table, seq_lens, *, window=None, k_sink=None, gate=None,
@@ -203,17 +247,7 @@ def paged_decode_attention(q, k_pages, v_pages, block_table, seq_lens, *, window
     """paged_prompt_attention for one new token per sequence: row s of q [num_seqs, H, hd] is the
     last token of sequence s.  The keys of a sequence are split over thread blocks and joined in a
     fixed order.  seq_lens[s] == 0 marks an empty slot: its row is zero."""
-    n, head, tail, o, keep = _attention_inputs(q, k_pages, v_pages, block_table, seq_lens, None, window, k_sink, gate,
-                                               scale)
-    lse = _lse_of(return_lse, o)
-    if n:
-        L = Z.lib()
-        ws = torch.empty(int(L.zs_paged_decode_workspace(n, o.size(1), k_pages.size(1), o.size(2))),
-                         dtype=torch.uint8, device=o.device)
-        Z.count(1)
-        Z.check(L.zs_paged_decode_attention(*head, n, *tail, Z.ptr(lse), Z.dtype_code(o.dtype), ws.data_ptr(),
-                                            ws.numel(), Z.stream_of(o)), "zs_paged_decode_attention")
-    return (o, lse) if return_lse else o
+    return _attention(q, k_pages, v_pages, block_table, seq_lens, None, window, k_sink, gate, scale, return_lse, True)
 
 
 class PagedKVCache:
@@ -231,13 +265,14 @@ class PagedKVCache:
     def __init__(self, n_layers, n_kv_heads, head_dim, *, num_pages, page_size=64, max_seqs, max_pages_per_seq,
                  dtype=torch.bfloat16, device="cuda"):
         device = torch.device(device)
-        _refuse(device.type != "cuda", f"the cache lives on a CUDA device (got {device})")
-        _refuse(dtype not in _DTYPES or page_size not in PAGE_SIZES or head_dim not in (64, 128),
-                f"the cache holds bf16 or f16 pages of {PAGE_SIZES} tokens of head_dim 64 or 128 (got {dtype}, "
-                f"{page_size}, {head_dim})")
-        _refuse(min(n_layers, n_kv_heads, num_pages, max_seqs, max_pages_per_seq) < 1 or num_pages > 2_000_000
-                or max_pages_per_seq * page_size >= 1 << 31,
-                "n_layers, n_kv_heads, num_pages (at most 2000000), max_seqs and max_pages_per_seq must be positive")
+        if device.type != "cuda":
+            _fail(f"the cache lives on a CUDA device (got {device})")
+        if dtype not in _DTYPES or page_size not in PAGE_SIZES or head_dim not in (64, 128):
+            _fail(f"the cache holds bf16 or f16 pages of {PAGE_SIZES} tokens of head_dim 64 or 128 (got {dtype}, "
+                  f"{page_size}, {head_dim})")
+        if (min(n_layers, n_kv_heads, num_pages, max_seqs, max_pages_per_seq) < 1 or num_pages > 2_000_000
+                or max_pages_per_seq * page_size >= 1 << 31):
+            _fail("n_layers, n_kv_heads, num_pages (at most 2000000), max_seqs and max_pages_per_seq must be positive")
         self.kv = torch.zeros(n_layers, 2, num_pages, n_kv_heads, page_size, head_dim, dtype=dtype, device=device)
         cells = max_seqs * max_pages_per_seq
         self.meta = torch.empty(cells + max_seqs + num_pages, dtype=torch.int32, device=device)
@@ -245,9 +280,10 @@ class PagedKVCache:
         self.seq_lens = self.meta[cells:cells + max_seqs]
         self.ref_count = self.meta[cells + max_seqs:]
         self.reset()
-        self._c = Z.KvCache(self.kv.data_ptr(), self.block_table.data_ptr(), self.seq_lens.data_ptr(),
-                            self.ref_count.data_ptr(), num_pages, n_layers, n_kv_heads, page_size, head_dim, max_seqs,
-                            max_pages_per_seq)
+        self._dev = self.kv.get_device()
+        self._c = ctypes.pointer(Z.KvCache(
+            self.kv.data_ptr(), self.block_table.data_ptr(), self.seq_lens.data_ptr(), self.ref_count.data_ptr(),
+            num_pages, n_layers, n_kv_heads, page_size, head_dim, max_seqs, max_pages_per_seq))
 
     @property
     def page_size(self):
@@ -273,52 +309,52 @@ class PagedKVCache:
                                    (0x40, "no free page, or a slot without room")) if err & b]
             raise Z.ZsError(f"paged cache: {'; '.join(what) or 'device error'} (device error word {err:#x})")
 
-    def _requests(self, *lists):
+    def _requests(self, lists):
         out = []
         for x in lists:
-            if isinstance(x, int):
-                x = [x]
             if not torch.is_tensor(x):
-                x = torch.tensor(list(x), dtype=torch.int32, device=self.kv.device)
-            _refuse(x.dtype != torch.int32 or x.dim() != 1 or not x.is_contiguous() or x.device != self.kv.device,
-                    f"requests are contiguous int32 [n] tensors on {self.kv.device} (got {x.dtype} {tuple(x.shape)} "
-                    f"on {x.device})")
+                x = torch.tensor([x] if isinstance(x, int) else list(x), dtype=torch.int32, device=self.kv.device)
+            if x.dtype != torch.int32 or x.dim() != 1 or not x.is_contiguous() or x.get_device() != self._dev:
+                _fail(f"requests are contiguous int32 [n] tensors on {self.kv.device} (got {x.dtype} "
+                      f"{tuple(x.shape)} on {x.device})")
             out.append(x)
-        _refuse(len({x.numel() for x in out}) != 1, "request lists must have one length")
+        if len(out) > 1 and out[0].shape != out[1].shape:
+            _fail("request lists must have one length")
         return out
 
-    def _workspace(self, n):
-        return torch.empty(int(Z.lib().zs_kv_workspace(ctypes.byref(self._c), n)), dtype=torch.uint8,
-                           device=self.kv.device)
-
     def _call(self, name, launches, *lists):
-        n = lists[0].numel() if lists else 0
+        lists = self._requests(lists)
+        n = lists[0].size(0) if lists else 0
         if lists and n == 0:
             return
-        ws = self._workspace(n)
+        L = Z.lib()
+        size = L.zs_kv_workspace(self._c, n)
+        ws = torch.empty(size, dtype=torch.uint8, device=self.kv.device)
+        args = [x.data_ptr() for x in lists]
+        if lists:
+            args.append(n)
         Z.count(launches)
-        args = [x.data_ptr() for x in lists] + ([n] if lists else [])
-        Z.check(getattr(Z.lib(), name)(ctypes.byref(self._c), *args, ws.data_ptr(), ws.numel(),
-                                       Z.stream_of(self.kv)), name)
+        rc = getattr(L, name)(self._c, *args, ws.data_ptr(), size, torch._C._cuda_getCurrentRawStream(self._dev))
+        if rc:
+            Z.check(rc, name)
 
     def extend(self, slots, n_tokens):
         """Slot slots[i] grows by n_tokens[i] >= 0 tokens, with pages for them; what they hold is
         up to the caller (paged_append).  A slot named twice grows by its first request only."""
-        self._call("zs_kv_extend", 1, *self._requests(slots, n_tokens))
+        self._call("zs_kv_extend", 1, slots, n_tokens)
 
     def fork(self, src, dst):
         """Slot dst[i] becomes a copy of slot src[i] as it was before the call (beam search:
         fork(parents, slots)); what dst[i] held is let go.  Whole pages are shared; the filled
         rows of a last partial page are copied into a page of dst[i]'s own."""
-        self._call("zs_kv_fork", 4, *self._requests(src, dst))
+        self._call("zs_kv_fork", 4, src, dst)
 
     def free(self, slots):
         """Slots become empty; pages that no slot holds any more are free."""
-        (s,) = self._requests(slots)
+        (s,) = self._requests([slots])
         if s.numel():
             Z.count(1)
-            Z.check(Z.lib().zs_kv_free(ctypes.byref(self._c), s.data_ptr(), s.numel(), Z.stream_of(self.kv)),
-                    "zs_kv_free")
+            Z.check(Z.lib().zs_kv_free(self._c, s.data_ptr(), s.numel(), Z.stream_of(self.kv)), "zs_kv_free")
 
     def compact(self):
         """The pages in use become pages 0 .. U-1 (the k-th free page below U takes the k-th used
@@ -328,4 +364,4 @@ class PagedKVCache:
     def copy_pages(self, src, dst):
         """Page dst[i] = page src[i], every layer's keys and values; the tables stay.  A page that
         is written must not also be read by the call."""
-        self._call("zs_kv_copy_pages", 2, *self._requests(src, dst))
+        self._call("zs_kv_copy_pages", 2, src, dst)
