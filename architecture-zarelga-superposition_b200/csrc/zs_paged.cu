@@ -49,15 +49,21 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
 }
 
 // The sequence of packed token t: the last s with cu[s] <= t (empty sequences
-// in between hold no token); -1 when t lies before cu[0] or from cu[n] on.
+// in between hold no token); -1 when t lies before cu[0] or from cu[n] on.  A
+// whole warp asks together: each round of the search reads 32 entries at once.
 __device__ __forceinline__ int sequence_of(const int* cu, int n, int t) {
-  if (t < __ldg(cu) || t >= __ldg(cu + n)) return -1;
-  int lo = 0, hi = n;   // cu[lo] <= t < cu[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (__ldg(cu + mid) <= t) lo = mid; else hi = mid;
+  const int lane = threadIdx.x & 31;
+  int lo = 0, w = n + 1;                   // the last entry <= t is one of cu[lo .. lo + w)
+  while (true) {
+    const int step = (w + 31) / 32, i = lane * step;
+    const uint32_t below = __ballot_sync(0xffffffffu, i < w && __ldg(cu + lo + i) <= t);
+    if (below == 0) return -1;             // only when t < cu[0]
+    const int j = (31 - __clz(below)) * step;
+    lo += j;
+    w = min(step, w - j);
+    if (step == 1) break;
   }
-  return lo;
+  return lo < n ? lo : -1;
 }
 
 // ---------------------------------------------------------------------------- append
@@ -91,18 +97,33 @@ struct AppendArgs {
 
 // One head row is hd / 8 lanes of 16 bytes, so a warp holds 256 / hd rows at a
 // time and every load and store is a 16-byte one.  A warp owns one of `parts`
-// shares of a token's rows; the token's sequence and page are looked up once.
-// HBM-bound: each projected value is read once and written once.
+// shares of a token's rows.  HBM-bound (each projected value is read once and
+// written once), so what matters is loads in flight: the first six rows are
+// asked for before the token's sequence and page are looked up, and a lane's
+// cos and sin are read once per token.
 template <typename T, int HD>
 __global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a) {
   constexpr int LPR = HD / 8;          // lanes per row
   constexpr int RPW = 32 / LPR;        // rows per warp pass
+  constexpr int AHEAD = 6;             // passes loaded together
   const int lane = threadIdx.x & 31;
   const int rl = lane % LPR, rs = lane / LPR;
   const int64_t item = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   if (item >= a.tokens * a.parts) return;
   const int64_t tok = item / a.parts;
   const int part = (int)(item - tok * a.parts);
+  const int rows = a.H + 2 * a.Hkv;
+  const T* x = reinterpret_cast<const T*>(a.x) + tok * a.ldx;
+  uint4 raw[AHEAD];
+  auto load = [&](int r0) {
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int r = r0 + u * a.parts * RPW + rs;
+      raw[u] = r < rows ? __ldcs(reinterpret_cast<const uint4*>(x + (int64_t)r * HD + rl * 8)) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  load(part * RPW);
+
   int seq = (int)tok;
   int64_t pos = -1;
   if (a.cu != nullptr) {
@@ -121,27 +142,33 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a) {
       live = false;
     }
   }
-  const int rows = a.H + 2 * a.Hkv;
-  const T* x = reinterpret_cast<const T*>(a.x) + tok * a.ldx;
   T* q = reinterpret_cast<T*>(a.q_out) + tok * (int64_t)a.H * HD;
   const int64_t at = live ? page * a.page_stride + (pos % a.page) * HD : 0;
   const int p0 = (rl % (LPR / 2)) * 8;           // pair index of this lane's first value
-  const bool low = rl < LPR / 2;
-#pragma unroll 2
-  for (int r0 = part * RPW; r0 < rows; r0 += a.parts * RPW) {
-    const int r = r0 + rs;
-    const bool in = r < rows;
-    const bool is_q = r < a.H;
-    const uint4 raw = in ? *reinterpret_cast<const uint4*>(x + (int64_t)r * HD + rl * 8) : make_uint4(0, 0, 0, 0);
-    float v[8];
-    unpack8<T>(raw, v);
-    if (a.wq != nullptr) {
-      float ss = 0.f;
+  float cs[8], sn[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(v[e], v[e], ss);
+  for (int e = 0; e < 8; ++e) {
+    const bool turn = live && p0 + e < a.rot;
+    cs[e] = turn ? __ldg(a.cos + pos * a.table_ld + p0 + e) : 1.f;
+    sn[e] = turn ? __ldg(a.sin + pos * a.table_ld + p0 + e) : 0.f;
+    if (rl < LPR / 2) sn[e] = -sn[e];
+  }
+  for (int r0 = part * RPW; r0 < rows; r0 += AHEAD * a.parts * RPW) {
+    if (r0 != part * RPW) load(r0);
 #pragma unroll
-      for (int off = LPR / 2; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-      if (r < a.H + a.Hkv) {
+    for (int u = 0; u < AHEAD; ++u) {
+      const int rb = r0 + u * a.parts * RPW;
+      if (rb >= rows) break;
+      const int r = rb + rs;
+      const bool is_q = r < a.H, is_k = !is_q && r < a.H + a.Hkv;
+      float v[8];
+      unpack8<T>(raw[u], v);
+      if (a.wq != nullptr) {
+        float ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss = fmaf(v[e], v[e], ss);
+#pragma unroll
+        for (int off = LPR / 2; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
         const float rstd = rsqrtf(ss / (float)HD + a.eps);
         const float4* w = reinterpret_cast<const float4*>((is_q ? a.wq : a.wk) + rl * 8);
         const float4 w0 = __ldg(w), w1 = __ldg(w + 1);
@@ -149,31 +176,21 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = (v[e] * rstd) * (1.0f + g[e]);
       }
-    }
-    if (a.rot > 0) {
-      float pv[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) pv[e] = __shfl_xor_sync(0xffffffffu, v[e], LPR / 2);
-      if (live && p0 < a.rot && r < a.H + a.Hkv) {
-        const float* c = a.cos + pos * a.table_ld + p0;
-        const float* s = a.sin + pos * a.table_ld + p0;
+      if (a.rot > 0) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          if (p0 + e < a.rot) {
-            const float cc = __ldg(c + e), sn = __ldg(s + e);
-            v[e] = low ? v[e] * cc - pv[e] * sn : v[e] * cc + pv[e] * sn;
-          }
+          const float pv = __shfl_xor_sync(0xffffffffu, v[e], LPR / 2);
+          if (p0 + e < a.rot) v[e] = v[e] * cs[e] + pv * sn[e];
         }
       }
-    }
-    if (!in) continue;
-    if (is_q) {
-      *reinterpret_cast<uint4*>(q + (int64_t)r * HD + rl * 8) = live ? pack8<T>(v) : make_uint4(0, 0, 0, 0);
-    } else if (live) {
-      const bool is_k = r < a.H + a.Hkv;
-      const int h = r - a.H - (is_k ? 0 : a.Hkv);
-      T* dst = reinterpret_cast<T*>(is_k ? a.k_pages : a.v_pages) + at + (int64_t)h * a.page * HD + rl * 8;
-      *reinterpret_cast<uint4*>(dst) = is_k ? pack8<T>(v) : raw;   // values keep their bits
+      if (r >= rows) continue;
+      if (is_q) {
+        *reinterpret_cast<uint4*>(q + (int64_t)r * HD + rl * 8) = live ? pack8<T>(v) : make_uint4(0, 0, 0, 0);
+      } else if (live) {
+        const int h = r - a.H - (is_k ? 0 : a.Hkv);
+        T* dst = reinterpret_cast<T*>(is_k ? a.k_pages : a.v_pages) + at + (int64_t)h * a.page * HD + rl * 8;
+        *reinterpret_cast<uint4*>(dst) = is_k ? pack8<T>(v) : raw[u];   // values keep their bits
+      }
     }
   }
 }
@@ -187,6 +204,8 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a) {
 // reads what another writes.
 
 constexpr int PLAN_THREADS = 1024;
+constexpr int PLAN_SLOTS = 8192;           // slots whose marks fit the plan's shared memory
+constexpr int PLAN_CELLS = 8192;           // table cells that one block rewrites as fast as a grid launched for them
 
 struct Plan {              // device workspace of a call, all int32
   int* count;              // number of moves
@@ -294,9 +313,10 @@ __device__ __forceinline__ void allot(const zs_kv_cache& c, const Plan& p, int n
   __syncthreads();
 }
 
-__global__ void __launch_bounds__(PLAN_THREADS) kv_extend_kernel(const zs_kv_cache c, const Plan p, const int* slots,
+__global__ void __launch_bounds__(PLAN_THREADS) kv_extend_kernel(const zs_kv_cache c, Plan p, const int* slots,
                                                                  const int* tokens, int n) {
-  __shared__ int s_warp[32];
+  __shared__ int s_warp[32], s_first[PLAN_SLOTS];
+  if (c.max_seqs <= PLAN_SLOTS) p.first = s_first;
   mark_first(slots, n, c.max_seqs, p.first);
   auto need_of = [&](int i) -> int {
     const int s = slots[i], t = tokens[i];
@@ -330,9 +350,28 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv_extend_kernel(const zs_kv_cac
   }
 }
 
-__global__ void __launch_bounds__(PLAN_THREADS) kv_fork_plan_kernel(const zs_kv_cache c, const Plan p, const int* src,
-                                                                    const int* dst, int n) {
-  __shared__ int s_warp[32];
+// Request i's cell j: the new row's page (the source's whole pages, then a page of its own
+// for the partial one), kept until every source row is read; the counts of what the
+// request holds and lets go.
+__device__ __forceinline__ void fork_cell(const zs_kv_cache& c, const Plan& p, const int* src, const int* dst, int i,
+                                          int j) {
+  const int full = p.len[i] / c.page_size;
+  const int old = c.block_table[(int64_t)dst[i] * c.max_pages + j];
+  int pg = -1;
+  if (j < full)
+    pg = c.block_table[(int64_t)src[i] * c.max_pages + j];
+  else if (j == full && p.len[i] % c.page_size)
+    pg = p.free_pages[p.off[i]];
+  if (j <= full && (pg >= 0 || j < full)) hold(c, pg, 1);
+  p.snap[(int64_t)i * c.max_pages + j] = pg;
+  if (old != -1) hold(c, old, -1);
+}
+
+__global__ void __launch_bounds__(PLAN_THREADS) kv_fork_plan_kernel(const zs_kv_cache c, Plan p, const int* src,
+                                                                    const int* dst, int n, int rows_here) {
+  __shared__ int s_warp[32], s_first[PLAN_SLOTS];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (c.max_seqs <= PLAN_SLOTS) p.first = s_first;
   mark_first(dst, n, c.max_seqs, p.first);
   auto need_of = [&](int i) -> int {
     const int s = src[i], d = dst[i];
@@ -369,37 +408,19 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv_fork_plan_kernel(const zs_kv_
     moves += sum;
   }
   if (threadIdx.x == 0) *p.count = moves;
-}
-
-// Block i: snapshot of request i's source row, counts of the pages it shares and lets go.
-__global__ void __launch_bounds__(128) kv_fork_count_kernel(const zs_kv_cache c, const Plan p, const int* src,
-                                                            const int* dst) {
-  const int i = blockIdx.x;
-  if (p.off[i] < 0) return;
-  const int full = p.len[i] / c.page_size;
-  const int* row = c.block_table + (int64_t)src[i] * c.max_pages;
-  const int* old = c.block_table + (int64_t)dst[i] * c.max_pages;
-  for (int j = threadIdx.x; j < c.max_pages; j += blockDim.x) {
-    int pg = -1;
-    if (j < full) {
-      pg = row[j];
-      hold(c, pg, 1);
-    } else if (j == full && p.len[i] % c.page_size) {
-      pg = p.free_pages[p.off[i]];
-      hold(c, pg, 1);
-    }
-    p.snap[(int64_t)i * c.max_pages + j] = pg;
-    if (old[j] != -1) hold(c, old[j], -1);
+  if (!rows_here) return;
+  for (int e = threadIdx.x; e < n * c.max_pages; e += PLAN_THREADS) {
+    const int i = e / c.max_pages;
+    if (p.off[i] >= 0) fork_cell(c, p, src, dst, i, e - i * c.max_pages);
   }
 }
 
-// Block i: request i's new row and length.
-__global__ void __launch_bounds__(128) kv_fork_write_kernel(const zs_kv_cache c, const Plan p, const int* dst) {
+// The same cells from a grid, block i request i.
+__global__ void __launch_bounds__(256) kv_fork_rows_kernel(const zs_kv_cache c, const Plan p, const int* src,
+                                                           const int* dst) {
   const int i = blockIdx.x;
   if (p.off[i] < 0) return;
-  for (int j = threadIdx.x; j < c.max_pages; j += blockDim.x)
-    c.block_table[(int64_t)dst[i] * c.max_pages + j] = p.snap[(int64_t)i * c.max_pages + j];
-  if (threadIdx.x == 0) c.seq_lens[dst[i]] = p.len[i];
+  for (int j = threadIdx.x; j < c.max_pages; j += blockDim.x) fork_cell(c, p, src, dst, i, j);
 }
 
 __global__ void __launch_bounds__(128) kv_free_kernel(const zs_kv_cache c, const int* slots) {
@@ -424,6 +445,7 @@ __global__ void __launch_bounds__(128) kv_free_kernel(const zs_kv_cache c, const
 
 __global__ void __launch_bounds__(PLAN_THREADS) kv_compact_plan_kernel(const zs_kv_cache c, const Plan p) {
   __shared__ int s_warp[32];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   constexpr int PER = 8;
   const int64_t P = c.num_pages;
   auto used_mask = [&](int64_t p0) -> uint32_t {
@@ -473,18 +495,12 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv_compact_plan_kernel(const zs_
   }
 }
 
-__global__ void __launch_bounds__(256) kv_rename_kernel(const zs_kv_cache c, const Plan p) {
-  const int U = p.off[0];
-  const int64_t n = (int64_t)c.max_seqs * c.max_pages;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x)
-    if (c.block_table[i] >= U && c.block_table[i] < c.num_pages) c.block_table[i] = p.map[c.block_table[i]];
-}
-
 // Moves given by the caller: pages out of range, a target named twice (the
 // first stands) and a target that is also a source are refused.
 __global__ void __launch_bounds__(PLAN_THREADS) kv_copy_plan_kernel(const zs_kv_cache c, const Plan p, const int* src,
                                                                     const int* dst, int n) {
   __shared__ int s_warp[32];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const unsigned P = (unsigned)c.num_pages;
   for (int i = threadIdx.x; i < n; i += PLAN_THREADS) {
     if ((unsigned)src[i] < P) p.map[src[i]] = 0;
@@ -521,10 +537,32 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv_copy_plan_kernel(const zs_kv_
   if (threadIdx.x == 0) *p.count = moves;
 }
 
-// One work item: one head's filled rows of one page of one layer's keys or
-// values, a contiguous run of rows * hd elements.  HBM-bound: read once,
-// written once.
-__global__ void __launch_bounds__(256) kv_copy_pages_kernel(const zs_kv_cache c, const Plan p) {
+// What follows a plan: the tables rewritten (FORK: the new rows; COMPACT: moved pages
+// renamed), then the page data.  One work item: one head's filled rows of one page of one
+// layer's keys or values, a contiguous run of rows * hd elements.  HBM-bound: read once,
+// written once.  Launched while the plan still runs; waits for its end.
+enum { AFTER_COPY, AFTER_FORK, AFTER_COMPACT };
+
+template <int AFTER>
+__global__ void __launch_bounds__(256) kv_apply_kernel(const zs_kv_cache c, const Plan p, const int* dst, int n) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int64_t me = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, all = (int64_t)gridDim.x * blockDim.x;
+  if (AFTER == AFTER_FORK) {
+    for (int64_t e = me; e < (int64_t)n * c.max_pages; e += all) {
+      const int i = (int)(e / c.max_pages);
+      if (p.off[i] < 0) continue;
+      const int j = (int)(e - (int64_t)i * c.max_pages);
+      c.block_table[(int64_t)dst[i] * c.max_pages + j] = p.snap[e];
+      if (j == 0) c.seq_lens[dst[i]] = p.len[i];
+    }
+  }
+  if (AFTER == AFTER_COMPACT) {
+    const int U = p.off[0];
+    for (int64_t e = me; e < (int64_t)c.max_seqs * c.max_pages; e += all) {
+      const int pg = c.block_table[e];
+      if (pg >= U && pg < c.num_pages) c.block_table[e] = p.map[pg];
+    }
+  }
   const int64_t run = (int64_t)c.page_size * c.head_dim / 8;        // 16-byte words of a whole run
   const int64_t page = run * c.n_kv_heads;
   const int64_t slabs = 2 * (int64_t)c.n_layers;
@@ -604,10 +642,26 @@ extern "C" size_t zs_kv_workspace(const zs_kv_cache* c, int64_t n) {
   ZS_BIND(c->kv);                                                             \
   const paged::Plan p = paged::carve(*c, n, workspace)
 
-static int launch_copy(const zs_kv_cache& c, const paged::Plan& p, cudaStream_t stream) {
-  paged::kv_copy_pages_kernel<<<num_sms() * 8, 256, 0, stream>>>(c, p);
-  ZS_CUDA_TRY(cudaGetLastError());
+// A kernel that may be scheduled while the one before it in the stream still runs (it waits for
+// that one's end itself).
+template <typename... P, typename... A>
+static int launch_after(void (*kernel)(P...), dim3 grid, dim3 block, cudaStream_t stream, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  ZS_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, P(args)...));
   return ZS_OK;
+}
+
+template <int AFTER>
+static int launch_apply(const zs_kv_cache& c, const paged::Plan& p, const int* dst, int64_t n, cudaStream_t stream) {
+  return launch_after(paged::kv_apply_kernel<AFTER>, dim3(num_sms() * 8), dim3(256), stream, c, p, dst, (int)n);
 }
 
 extern "C" int zs_kv_extend(const zs_kv_cache* c, const int* slots, const int* tokens, int64_t n, void* workspace,
@@ -625,13 +679,14 @@ extern "C" int zs_kv_fork(const zs_kv_cache* c, const int* src, const int* dst, 
   ZS_KV_ENTER(n);
   if (n == 0) return ZS_OK;
   ZS_REQUIRE(src && dst, ZS_ERR_ARG);
-  paged::kv_fork_plan_kernel<<<1, paged::PLAN_THREADS, 0, stream>>>(*c, p, src, dst, (int)n);
+  const bool rows_here = n * c->max_pages <= paged::PLAN_CELLS;
+  paged::kv_fork_plan_kernel<<<1, paged::PLAN_THREADS, 0, stream>>>(*c, p, src, dst, (int)n, rows_here ? 1 : 0);
   ZS_CUDA_TRY(cudaGetLastError());
-  paged::kv_fork_count_kernel<<<(unsigned)n, 128, 0, stream>>>(*c, p, src, dst);
-  ZS_CUDA_TRY(cudaGetLastError());
-  paged::kv_fork_write_kernel<<<(unsigned)n, 128, 0, stream>>>(*c, p, dst);
-  ZS_CUDA_TRY(cudaGetLastError());
-  return launch_copy(*c, p, stream);
+  if (!rows_here) {
+    paged::kv_fork_rows_kernel<<<(unsigned)n, 256, 0, stream>>>(*c, p, src, dst);
+    ZS_CUDA_TRY(cudaGetLastError());
+  }
+  return launch_apply<paged::AFTER_FORK>(*c, p, dst, n, stream);
 }
 
 extern "C" int zs_kv_free(const zs_kv_cache* c, const int* slots, int64_t n, void* stream_) {
@@ -651,11 +706,7 @@ extern "C" int zs_kv_compact(const zs_kv_cache* c, void* workspace, size_t works
   ZS_KV_ENTER(0);
   paged::kv_compact_plan_kernel<<<1, paged::PLAN_THREADS, 0, stream>>>(*c, p);
   ZS_CUDA_TRY(cudaGetLastError());
-  const int64_t cells = (int64_t)c->max_seqs * c->max_pages;
-  const int64_t blocks = (cells + 255) / 256;
-  paged::kv_rename_kernel<<<(unsigned)(blocks < 592 ? blocks : 592), 256, 0, stream>>>(*c, p);
-  ZS_CUDA_TRY(cudaGetLastError());
-  return launch_copy(*c, p, stream);
+  return launch_apply<paged::AFTER_COMPACT>(*c, p, nullptr, 0, stream);
 }
 
 extern "C" int zs_kv_copy_pages(const zs_kv_cache* c, const int* src, const int* dst, int64_t n, void* workspace,
@@ -665,7 +716,7 @@ extern "C" int zs_kv_copy_pages(const zs_kv_cache* c, const int* src, const int*
   ZS_REQUIRE(src && dst, ZS_ERR_ARG);
   paged::kv_copy_plan_kernel<<<1, paged::PLAN_THREADS, 0, stream>>>(*c, p, src, dst, (int)n);
   ZS_CUDA_TRY(cudaGetLastError());
-  return launch_copy(*c, p, stream);
+  return launch_apply<paged::AFTER_COPY>(*c, p, nullptr, 0, stream);
 }
 
 // Checks shared by the operators that read or write one layer's pages.

@@ -163,7 +163,7 @@ struct DecSmem {
   static constexpr int ALLOC = TOTAL + 1024;
 };
 
-// Partial results: [block][2][16 rows][HD + 2] (O, max, sum), then the running tile counts.
+// Partial results: [block][2] of O [16 rows][HD] and (max, sum) [16 rows].
 __host__ __device__ constexpr int64_t part_floats(int hd) { return (int64_t)DEC_ROWS * (hd + 2); }
 
 struct Span {              // the key tiles of a sequence
@@ -223,19 +223,46 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, u
       : "memory");
 }
 
-// The sink's logit of query head h (log2 units), summed over the 8 lanes that call together.
-template <typename T, int HD>
-__device__ __forceinline__ float sink_logit8(const AttnArgs& a, int64_t tok, int h) {
-  const int part = threadIdx.x & 7;
+// N consecutive values of the sink from element i (a multiple of N).
+template <int N>
+__device__ __forceinline__ void load_sink(const AttnArgs& a, int64_t i, float (&v)[N]) {
+  static_assert(N == 4, "4 values a lane");
+  if (a.sink_dtype == ZS_F32) {
+    const float4 x = __ldg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(a.k_sink) + i));
+    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+  } else {
+    const uint2 x = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(a.k_sink) + i));
+    const uint32_t w[2] = {x.x, x.y};
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float2 f = a.sink_dtype == ZS_BF16 ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[e]))
+                                               : __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+      v[2 * e] = f.x, v[2 * e + 1] = f.y;
+    }
+  }
+}
+
+// The sink's logit of query head h (log2 units), summed over LANES neighbouring lanes that call
+// together (all of the warp's lanes call).
+template <typename T, int HD, int LANES>
+__device__ __forceinline__ float sink_logit(const AttnArgs& a, int64_t tok, int h) {
+  const int part = threadIdx.x & (LANES - 1);
   const T* q = reinterpret_cast<const T*>(a.q) + tok * a.ldq + (int64_t)h * HD;
   float dot = 0.f;
 #pragma unroll
-  for (int e = 0; e < HD / 8; ++e) {
-    const int c = part * (HD / 8) + e;
-    dot = fmaf(to_f32(q[c]), load_any(a.k_sink, a.sink_dtype, (int64_t)h * HD + c), dot);
+  for (int c = part * 4; c < HD; c += LANES * 4) {
+    const uint2 x = *reinterpret_cast<const uint2*>(q + c);
+    const float2 f0 = Pair<T>::to_f(*reinterpret_cast<const typename Pair<T>::type*>(&x.x));
+    const float2 f1 = Pair<T>::to_f(*reinterpret_cast<const typename Pair<T>::type*>(&x.y));
+    float v[4];
+    load_sink<4>(a, (int64_t)h * HD + c, v);
+    dot = fmaf(f0.x, v[0], dot);
+    dot = fmaf(f0.y, v[1], dot);
+    dot = fmaf(f1.x, v[2], dot);
+    dot = fmaf(f1.y, v[3], dot);
   }
 #pragma unroll
-  for (int off = 4; off > 0; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
+  for (int off = LANES / 2; off > 0; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
   return dot * a.scale_log2;
 }
 
@@ -519,8 +546,8 @@ __global__ void __launch_bounds__(160, 2)
     const bool whole = from_start && to_end;
     const int row = threadIdx.x >> 3, col = (threadIdx.x & 7) * 4;
     const int h = h0 + min(row, nrow - 1);
-    const float z = whole && a.k_sink != nullptr ? sink_logit8<T, HD>(a, pseq, h) : 0.f;
-    float* part = parts + ((int64_t)blockIdx.x * 2 + (first ? 0 : 1)) * part_floats(HD) + row * (HD + 2);
+    const float z = whole && a.k_sink != nullptr ? sink_logit<T, HD, 8>(a, pseq, h) : 0.f;
+    float* part = parts + ((int64_t)blockIdx.x * 2 + (first ? 0 : 1)) * part_floats(HD);
     bool stop = false;
 #pragma unroll
     for (int ps = 0; ps < HD / 32; ++ps) {             // 32 columns at a time
@@ -549,10 +576,8 @@ __global__ void __launch_bounds__(160, 2)
         if (whole) {
           finish_row<T, HD>(a, pseq, h, ps * 32 + col, mt, lt, acc, z, ps == 0 && col == 0);
         } else {
-          float2* dst = reinterpret_cast<float2*>(part + ps * 32 + col);
-          dst[0] = make_float2(acc[0], acc[1]);
-          dst[1] = make_float2(acc[2], acc[3]);
-          if (ps == 0 && col == 0) *reinterpret_cast<float2*>(part + HD) = make_float2(mt, lt);
+          *reinterpret_cast<float4*>(part + row * HD + ps * 32 + col) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+          if (ps == 0 && col == 0) *reinterpret_cast<float2*>(part + DEC_ROWS * HD + row * 2) = make_float2(mt, lt);
         }
       }
       stop = consumer_any(*s_abort);                   // also: the buffer may be written again
@@ -566,10 +591,16 @@ __global__ void __launch_bounds__(160, 2)
 }
 
 // Block (sequence, unit): the sum of its parts, where more than one block of the decode
-// kernel had a part of it.
+// kernel had a part of it.  A warp takes a row (four columns a lane) or, when the rows are
+// few, one of several shares of a row's parts; it keeps four parts' loads in flight.
+constexpr int JOIN_WARPS = 8;
+
 template <typename T, int HD>
-__global__ void __launch_bounds__(128) paged_join_kernel(const AttnArgs a, const float* parts, const int64_t* counts,
-                                                         int decode_blocks) {
+__global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const AttnArgs a, const float* parts,
+                                                                     const int64_t* counts, int decode_blocks) {
+  constexpr int SUB = 128 / HD;            // parts side by side in a warp
+  __shared__ float s_o[JOIN_WARPS][HD], s_ml[JOIN_WARPS][2];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = a.H / a.Hkv;
   const int blocks_g = (G + DEC_ROWS - 1) / DEC_ROWS;
   const int units = a.Hkv * blocks_g;
@@ -577,38 +608,82 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const AttnArgs a, const
   const int hk = unit / blocks_g, g0 = (unit - hk * blocks_g) * DEC_ROWS;
   const int h0 = hk * G + g0, nrow = min(DEC_ROWS, G - g0);
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int64_t before = counts[seq], tiles = counts[seq + 1] - before;
   const int64_t all = counts[a.num_seqs] * units, nb = min((int64_t)decode_blocks, all);
-  const int64_t tiles = counts[seq + 1] - counts[seq];
-  const int64_t t0 = counts[seq] * units + unit * tiles, t1 = t0 + tiles - 1;
+  const int64_t t0 = before * units + unit * tiles, t1 = t0 + tiles - 1;
   // block of tile t: the last b with floor(b * all / nb) <= t
-  const int64_t b0 = ((t0 + 1) * nb - 1) / all, b1 = ((t1 + 1) * nb - 1) / all;
+  const int b0 = (int)(((t0 + 1) * nb - 1) / all), b1 = (int)(((t1 + 1) * nb - 1) / all);
   if (b0 == b1) return;
-  const int row = threadIdx.x >> 3;
-  const int h = h0 + min(row, nrow - 1);
-  const float z = a.k_sink != nullptr ? sink_logit8<T, HD>(a, seq, h) : 0.f;
-  if (row >= nrow) return;
-  auto part_of = [&](int64_t b) {
-    // a block's first part lies in its slot 0; one that starts inside the block's run in slot 1
-    return parts + (b * 2 + (b * all / nb < t0 ? 1 : 0)) * part_floats(HD) + row * (HD + 2);
-  };
-  float mt = -INFINITY;
-  for (int64_t b = b0; b <= b1; ++b) mt = fmaxf(mt, part_of(b)[HD]);
+  // a block's first part lies in its slot 0; one that starts inside the block's run (only the
+  // first can) in slot 1
+  const int shift = b0 * all / nb < t0 ? 1 : 0;
+  const int shares = nrow >= JOIN_WARPS ? 1 : JOIN_WARPS / nrow;
+  const int share = warp % shares, sub = lane / (HD / 4), col = (lane % (HD / 4)) * 4;
+  for (int row = warp / shares; row < nrow; row += JOIN_WARPS / shares) {
+    float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+    const int step = shares * SUB;
+    for (int b = b0 + share * SUB + sub; b <= b1; b += 4 * step) {
+      float4 o[4];
+      float2 ml[4];
 #pragma unroll
-  for (int ps = 0; ps < HD / 32; ++ps) {
-    const int col = ps * 32 + (threadIdx.x & 7) * 4;
-    float lt = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int64_t b = b0; b <= b1; ++b) {
-      const float* part = part_of(b);
-      const float mw = part[HD], fw = mw == -INFINITY ? 0.f : exp2f(mw - mt);
-      lt = fmaf(fw, part[HD + 1], lt);
-      const float2 x = *reinterpret_cast<const float2*>(part + col), y = *reinterpret_cast<const float2*>(part + col + 2);
-      acc[0] = fmaf(fw, x.x, acc[0]);
-      acc[1] = fmaf(fw, x.y, acc[1]);
-      acc[2] = fmaf(fw, y.x, acc[2]);
-      acc[3] = fmaf(fw, y.y, acc[3]);
+      for (int e = 0; e < 4; ++e) {
+        const int bb = b + e * step;
+        ml[e] = make_float2(-INFINITY, 0.f);
+        o[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (bb <= b1) {
+          const float* part = parts + ((int64_t)bb * 2 + (bb == b0 ? shift : 0)) * part_floats(HD);
+          ml[e] = *reinterpret_cast<const float2*>(part + DEC_ROWS * HD + row * 2);
+          o[e] = *reinterpret_cast<const float4*>(part + row * HD + col);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float mt = fmaxf(m, ml[e].x);
+        const float f = m == -INFINITY ? 0.f : exp2f(m - mt), fe = ml[e].x == -INFINITY ? 0.f : exp2f(ml[e].x - mt);
+        l = l * f + ml[e].y * fe;
+        acc[0] = acc[0] * f + o[e].x * fe;
+        acc[1] = acc[1] * f + o[e].y * fe;
+        acc[2] = acc[2] * f + o[e].z * fe;
+        acc[3] = acc[3] * f + o[e].w * fe;
+        m = mt;
+      }
     }
-    finish_row<T, HD>(a, seq, h, col, mt, lt, acc, z, col == 0);
+    if (SUB == 2) {                        // the two halves of the warp, the lower first
+      const float mo = __shfl_xor_sync(0xffffffffu, m, 16), lo = __shfl_xor_sync(0xffffffffu, l, 16);
+      const float mt = fmaxf(m, mo);
+      const float f = m == -INFINITY ? 0.f : exp2f(m - mt), fo = mo == -INFINITY ? 0.f : exp2f(mo - mt);
+      l = l * f + lo * fo;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] = acc[e] * f + __shfl_xor_sync(0xffffffffu, acc[e], 16) * fo;
+      m = mt;
+    }
+    if (shares > 1) {                      // then every warp is here once
+      if (sub == 0) *reinterpret_cast<float4*>(&s_o[warp][col]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      if (lane == 0) {
+        s_ml[warp][0] = m;
+        s_ml[warp][1] = l;
+      }
+    } else {
+      const int h = h0 + row;
+      const float z = a.k_sink != nullptr ? sink_logit<T, HD, 32>(a, seq, h) : 0.f;
+      if (sub == 0) finish_row<T, HD>(a, seq, h, col, m, l, acc, z, col == 0);
+    }
   }
+  if (shares == 1) return;
+  __syncthreads();
+  const int row = warp / shares;
+  if (share != 0 || row >= nrow) return;
+  const int h = h0 + row;
+  const float z = a.k_sink != nullptr ? sink_logit<T, HD, 32>(a, seq, h) : 0.f;
+  float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int w = warp; w < warp + shares; ++w) m = fmaxf(m, s_ml[w][0]);
+  for (int w = warp; w < warp + shares; ++w) {
+    const float f = s_ml[w][0] == -INFINITY ? 0.f : exp2f(s_ml[w][0] - m);
+    l = fmaf(f, s_ml[w][1], l);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] = fmaf(f, s_o[w][col + e], acc[e]);
+  }
+  if (sub == 0) finish_row<T, HD>(a, seq, h, col, m, l, acc, z, col == 0);
 }
 
 }  // namespace paged
@@ -628,6 +703,7 @@ static int attn_args(paged::AttnArgs& a, const void* q, int64_t ldq, const void*
   ZS_REQUIRE(window >= 0 && ldq >= (int64_t)H * hd && (gate == nullptr || ldg >= H), ZS_ERR_SHAPE);
   ZS_REQUIRE(ldq % 8 == 0 && ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(o)) & 15) == 0, ZS_ERR_ALIGN);
   ZS_REQUIRE(k_sink == nullptr || sink_dtype == ZS_F32 || sink_dtype == ZS_BF16 || sink_dtype == ZS_F16, ZS_ERR_DTYPE);
+  ZS_REQUIRE((reinterpret_cast<uintptr_t>(k_sink) & 15) == 0, ZS_ERR_ALIGN);
   a.q = q;
   a.ldq = ldq;
   a.k_pages = k_pages;
@@ -710,18 +786,8 @@ static int launch_decode(const paged::AttnArgs& a, int dtype, void* workspace, c
   paged::paged_decode_kernel<T, HD><<<blocks, 160, L::ALLOC, stream>>>(tk, tv, a, parts, counts);
   ZS_CUDA_TRY(cudaGetLastError());
   if (most == 1) return ZS_OK;                         // nothing can be split
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)a.num_seqs, (unsigned)units);
-  cfg.blockDim = dim3(128);
-  cfg.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  ZS_CUDA_TRY(cudaLaunchKernelEx(&cfg, paged::paged_join_kernel<T, HD>, a, (const float*)parts,
-                                 (const int64_t*)counts, blocks));
-  return ZS_OK;
+  return launch_after(paged::paged_join_kernel<T, HD>, dim3((unsigned)a.num_seqs, (unsigned)units),
+                      dim3(paged::JOIN_WARPS * 32), stream, a, parts, counts, blocks);
 }
 
 extern "C" size_t zs_paged_decode_workspace(int num_seqs, int H, int Hkv, int hd) {

@@ -191,6 +191,8 @@ def _attention(q, k_pages, v_pages, block_table, seq_lens, cu_seqlens, window, k
             _fail(f"k_sink must be [{H}, {hd}] (got {tuple(k_sink.shape)})")
         if not k_sink.is_contiguous():
             k_sink = k_sink.contiguous()
+        if k_sink.data_ptr() % 16:
+            k_sink = k_sink.clone()
         sink_dtype = Z.dtype_code(k_sink.dtype)
     ldg = 0
     if gate is not None:
@@ -347,7 +349,7 @@ class PagedKVCache:
         """Slot dst[i] becomes a copy of slot src[i] as it was before the call (beam search:
         fork(parents, slots)); what dst[i] held is let go.  Whole pages are shared; the filled
         rows of a last partial page are copied into a page of dst[i]'s own."""
-        self._call("zs_kv_fork", 4, src, dst)
+        self._call("zs_kv_fork", 2, src, dst)
 
     def free(self, slots):
         """Slots become empty; pages that no slot holds any more are free."""
@@ -359,7 +361,7 @@ class PagedKVCache:
     def compact(self):
         """The pages in use become pages 0 .. U-1 (the k-th free page below U takes the k-th used
         page from U on), so everything held lies in one run at the start of the pool."""
-        self._call("zs_kv_compact", 3)
+        self._call("zs_kv_compact", 2)
 
     def copy_pages(self, src, dst):
         """Page dst[i] = page src[i], every layer's keys and values; the tables stay.  A page that
