@@ -95,31 +95,49 @@ struct AppendArgs {
   int parts;                 // warps per token
 };
 
-// One head row is hd / 8 lanes of 16 bytes, so a warp holds 256 / hd rows at a
-// time and every load and store is a 16-byte one.  A warp owns one of `parts`
-// shares of a token's rows.  HBM-bound (each projected value is read once and
-// written once), so what matters is loads in flight: the first six rows are
-// asked for before the token's sequence and page are looked up, and a lane's
+// A warp holds 256 / hd head rows at a time; a lane has four columns of a row's
+// first half and the same four of its second half (8-byte accesses, whole
+// sectors), so it owns both members of the pairs that rotate.  A warp owns one
+// of `parts` shares of a token's rows.  HBM-bound (each projected value is read
+// once and written once), so what matters is loads in flight: the first rows
+// are asked for before the token's sequence and page are looked up, and gains,
 // cos and sin are read once per token.
+template <typename T>
+__device__ __forceinline__ void unpack4(const uint2& u, float* v) {
+  const float2 a = Pair<T>::to_f(*reinterpret_cast<const typename Pair<T>::type*>(&u.x));
+  const float2 b = Pair<T>::to_f(*reinterpret_cast<const typename Pair<T>::type*>(&u.y));
+  v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+}
+template <typename T>
+__device__ __forceinline__ uint2 pack4(const float* v) {
+  const typename Pair<T>::type a = Pair<T>::from_f(v[0], v[1]), b = Pair<T>::from_f(v[2], v[3]);
+  return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+
 template <typename T, int HD>
-__global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(256, 3) paged_append_kernel(const AppendArgs a) {
   constexpr int LPR = HD / 8;          // lanes per row
   constexpr int RPW = 32 / LPR;        // rows per warp pass
-  constexpr int AHEAD = 6;             // passes loaded together
+  constexpr int AHEAD = 4;             // passes loaded together
   const int lane = threadIdx.x & 31;
   const int rl = lane % LPR, rs = lane / LPR;
   const int64_t item = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   if (item >= a.tokens * a.parts) return;
   const int64_t tok = item / a.parts;
   const int part = (int)(item - tok * a.parts);
-  const int rows = a.H + 2 * a.Hkv;
-  const T* x = reinterpret_cast<const T*>(a.x) + tok * a.ldx;
-  uint4 raw[AHEAD];
+  const int rows = a.H + 2 * a.Hkv, turned = a.H + a.Hkv;
+  const int stride = a.parts * RPW;
+  const T* x = reinterpret_cast<const T*>(a.x) + tok * a.ldx + rl * 4;
+  uint2 lo[AHEAD], hi[AHEAD];
   auto load = [&](int r0) {
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
-      const int r = r0 + u * a.parts * RPW + rs;
-      raw[u] = r < rows ? __ldcs(reinterpret_cast<const uint4*>(x + (int64_t)r * HD + rl * 8)) : make_uint4(0, 0, 0, 0);
+      const int r = r0 + u * stride + rs;
+      lo[u] = hi[u] = make_uint2(0, 0);
+      if (r < rows) {
+        lo[u] = __ldcs(reinterpret_cast<const uint2*>(x + r * HD));
+        hi[u] = __ldcs(reinterpret_cast<const uint2*>(x + r * HD + HD / 2));
+      }
     }
   };
   load(part * RPW);
@@ -135,62 +153,75 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a) {
   int page = -1;
   bool live = pos >= 0;                // no sequence or a negative position: zero q, nothing stored
   if (live) {
-    const int64_t pi = pos / a.page;
+    const int pi = (int)pos / a.page;  // positions lie below 2^31
     if (pi < a.max_pages && (a.rot == 0 || pos < a.table_rows)) page = __ldg(a.block_table + seq * a.bt_ld + pi);
     if (page < 0 || page >= a.num_pages) {
       if (lane == 0 && part == 0) record_error(ZS_DEVERR_INDEX);
       live = false;
     }
   }
-  T* q = reinterpret_cast<T*>(a.q_out) + tok * (int64_t)a.H * HD;
-  const int64_t at = live ? page * a.page_stride + (pos % a.page) * HD : 0;
-  const int p0 = (rl % (LPR / 2)) * 8;           // pair index of this lane's first value
-  float cs[8], sn[8];
+  const int pairs = live ? min(a.rot - rl * 4, 4) : 0;   // pairs of this lane that rotate
+  float cs[4], sn[4];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const bool turn = live && p0 + e < a.rot;
-    cs[e] = turn ? __ldg(a.cos + pos * a.table_ld + p0 + e) : 1.f;
-    sn[e] = turn ? __ldg(a.sin + pos * a.table_ld + p0 + e) : 0.f;
-    if (rl < LPR / 2) sn[e] = -sn[e];
+  for (int e = 0; e < 4; ++e) {
+    cs[e] = e < pairs ? __ldg(a.cos + pos * a.table_ld + rl * 4 + e) : 1.f;
+    sn[e] = e < pairs ? __ldg(a.sin + pos * a.table_ld + rl * 4 + e) : 0.f;
   }
-  for (int r0 = part * RPW; r0 < rows; r0 += AHEAD * a.parts * RPW) {
+  T* q = reinterpret_cast<T*>(a.q_out) + tok * (int64_t)a.H * HD + rl * 4;
+  const int64_t at = live ? page * a.page_stride + (int)pos % a.page * HD + rl * 4 : 0;
+  T* kp = reinterpret_cast<T*>(a.k_pages) + at;
+  T* vp = reinterpret_cast<T*>(a.v_pages) + at;
+  for (int r0 = part * RPW; r0 < rows; r0 += AHEAD * stride) {
     if (r0 != part * RPW) load(r0);
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
-      const int rb = r0 + u * a.parts * RPW;
+      const int rb = r0 + u * stride;
       if (rb >= rows) break;
       const int r = rb + rs;
-      const bool is_q = r < a.H, is_k = !is_q && r < a.H + a.Hkv;
-      float v[8];
-      unpack8<T>(raw[u], v);
-      if (a.wq != nullptr) {
-        float ss = 0.f;
+      if (rb < turned) {                         // the warp has a query or key row
+        float v[8];
+        unpack4<T>(lo[u], v);
+        unpack4<T>(hi[u], v + 4);
+        if (a.wq != nullptr) {
+          float ss = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(v[e], v[e], ss);
+          for (int e = 0; e < 8; ++e) ss = fmaf(v[e], v[e], ss);
 #pragma unroll
-        for (int off = LPR / 2; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-        const float rstd = rsqrtf(ss / (float)HD + a.eps);
-        const float4* w = reinterpret_cast<const float4*>((is_q ? a.wq : a.wk) + rl * 8);
-        const float4 w0 = __ldg(w), w1 = __ldg(w + 1);
-        const float g[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+          for (int off = LPR / 2; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
+          const float rstd = rsqrtf(ss / (float)HD + a.eps);
+          const float* w = (r < a.H ? a.wq : a.wk) + rl * 4;
+          const float4 w0 = __ldg(reinterpret_cast<const float4*>(w));
+          const float4 w1 = __ldg(reinterpret_cast<const float4*>(w + HD / 2));
+          const float g[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = (v[e] * rstd) * (1.0f + g[e]);
-      }
-      if (a.rot > 0) {
+          for (int e = 0; e < 8; ++e) v[e] = (v[e] * rstd) * (1.0f + g[e]);
+        }
+        if (pairs > 0) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float pv = __shfl_xor_sync(0xffffffffu, v[e], LPR / 2);
-          if (p0 + e < a.rot) v[e] = v[e] * cs[e] + pv * sn[e];
+          for (int e = 0; e < 4; ++e) {
+            if (e < pairs) {
+              const float x1 = v[e], x2 = v[4 + e];
+              v[e] = x1 * cs[e] - x2 * sn[e];
+              v[4 + e] = x2 * cs[e] + x1 * sn[e];
+            }
+          }
+        }
+        if (r < turned) {                        // values keep their bits
+          lo[u] = pack4<T>(v);
+          hi[u] = pack4<T>(v + 4);
         }
       }
       if (r >= rows) continue;
-      if (is_q) {
-        *reinterpret_cast<uint4*>(q + (int64_t)r * HD + rl * 8) = live ? pack8<T>(v) : make_uint4(0, 0, 0, 0);
-      } else if (live) {
-        const int h = r - a.H - (is_k ? 0 : a.Hkv);
-        T* dst = reinterpret_cast<T*>(is_k ? a.k_pages : a.v_pages) + at + (int64_t)h * a.page * HD + rl * 8;
-        *reinterpret_cast<uint4*>(dst) = is_k ? pack8<T>(v) : raw[u];   // values keep their bits
+      T* dst;
+      if (r < a.H) {
+        dst = q + r * HD;
+        if (!live) lo[u] = hi[u] = make_uint2(0, 0);
+      } else {
+        if (!live) continue;
+        dst = r < turned ? kp + (int64_t)(r - a.H) * a.page * HD : vp + (int64_t)(r - turned) * a.page * HD;
       }
+      *reinterpret_cast<uint2*>(dst) = lo[u];
+      *reinterpret_cast<uint2*>(dst + HD / 2) = hi[u];
     }
   }
 }

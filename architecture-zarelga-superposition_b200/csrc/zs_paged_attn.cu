@@ -132,28 +132,33 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const AttnArgs a) {
 // ------------------------------------------------------------------------ decode
 //
 // One token per sequence: the cache is read once and hardly anything is computed, so the
-// kernel is bound by HBM.  The work is the list of 64-key tiles of every (sequence, key head,
-// block of 16 query heads), in that order, cut into equal runs, one per block: a batch of
-// sequences of any lengths loads every SM alike.  A block walks its run, and whatever part of
-// a (sequence, head) ends in it is finished there; parts of one that several blocks share go
-// to the workspace (at most two per block, the run's first and last) and
-// paged_join_kernel adds them in the order of the blocks.
+// kernel is bound by HBM.  The work is the list of 16 KiB key tiles of every unit (sequence,
+// key head, block of 16 query heads), in that order, cut into equal runs, one per block: a
+// batch of sequences of any lengths loads every SM alike.  A unit counts OVER steps more than
+// it has tiles, because its start and end (queries in, rows out) cost as much as that many.
+// A block walks its run, and whatever part of a unit ends in it is finished there; parts of
+// one that several blocks share go to the workspace (at most two per block, the run's first
+// and last) and paged_join_kernel adds them in the order of the blocks.
 //
 // Warp 4 loads the pages of a tile with TMA (128-byte swizzle) into a ring of stages; warps
-// 0-3 each take 16 of its keys: S = Q K^T and O += P V by mma.sync with the group's query heads
+// 0-3 each take a quarter of its keys: S = Q K^T and O += P V by mma.sync with the group's query heads
 // as the 16 rows, P straight from the accumulators of S, and a running (max, sum, O) of their
 // own, joined through shared memory when a part ends.  mma.sync, not tcgen05: a 128-row tile
 // would hold 1 to 16 rows of work, and the products are a tenth of the time of the loads.
 
-constexpr int DEC_TILE = 64;              // keys per tile
 constexpr int DEC_MAX_BLOCKS = 320;       // two per SM
 constexpr int DEC_ROWS = 16;              // query heads per block of rows
 constexpr int DEC_LDO = 40;               // floats per row of the join buffer (32 + padding against bank conflicts)
 
 template <int HD>
 struct DecSmem {
-  static constexpr int STAGES = HD == 128 ? 3 : 6;
-  static constexpr int MAT = DEC_TILE * HD * 2;                 // K or V of one tile
+  static constexpr int TILE = HD == 128 ? 64 : 128;             // keys per tile
+  // Steps of a unit's start and end, measured over 0 to 6: 32 sequences of 1 to 4096 tokens of 12/4
+  // heads of 128 take 42.5 us without, 33.1, 32.0, 31.7 and 32.3 us with 1 to 4; 129 windows of
+  // 512 of 16/4 heads of 64 take 23.4 us with 1 and 23.9 to 24.4 us with 2 to 6.
+  static constexpr int OVER = HD == 128 ? 3 : 1;
+  static constexpr int STAGES = 3;
+  static constexpr int MAT = TILE * HD * 2;                     // K or V of one tile
   static constexpr int STAGE = 2 * MAT;
   static constexpr int OFF_O = STAGES * STAGE;                  // [4 warps][16 rows][32 columns] f32, padded rows
   static constexpr int OFF_ML = OFF_O + 4 * DEC_ROWS * DEC_LDO * 4;  // max and sum [2][4][16]
@@ -163,20 +168,22 @@ struct DecSmem {
   static constexpr int ALLOC = TOTAL + 1024;
 };
 
-// Partial results: [block][2] of O [16 rows][HD] and (max, sum) [16 rows].
-__host__ __device__ constexpr int64_t part_floats(int hd) { return (int64_t)DEC_ROWS * (hd + 2); }
+// Partial results: [block][2] of O [rows][HD] and (max, sum) [rows], rows = min(group, 16).
+__host__ __device__ __forceinline__ int part_rows(int G) { return G < DEC_ROWS ? (G + 1) & ~1 : DEC_ROWS; }
+__host__ __device__ __forceinline__ int64_t part_floats(int hd, int rows) { return (int64_t)rows * (hd + 2); }
 
 struct Span {              // the key tiles of a sequence
   int len, first_key, first_tile, tiles;
 };
+template <int TILE>
 __device__ __forceinline__ Span span_of(const AttnArgs& a, int seq) {
   Span s;
   const int len = cut_length(a, seq);
   s.len = len > 0 ? len : 0;
   s.first_key = a.window > 0 && s.len > a.window ? s.len - a.window : 0;
-  s.first_tile = s.first_key / DEC_TILE;
+  s.first_tile = s.first_key / TILE;
   // an empty sequence has one tile with no key in it, so that its rows are written
-  s.tiles = max((s.len + DEC_TILE - 1) / DEC_TILE - s.first_tile, 1);
+  s.tiles = max((s.len + TILE - 1) / TILE - s.first_tile, 1);
   return s;
 }
 
@@ -266,10 +273,16 @@ __device__ __forceinline__ float sink_logit(const AttnArgs& a, int64_t tok, int 
   return dot * a.scale_log2;
 }
 
+template <typename T>
+__device__ __forceinline__ float gate_of(const AttnArgs& a, int64_t tok, int h) {
+  if (a.gate == nullptr) return 1.f;
+  return 1.f / (1.f + expf(-to_f32(reinterpret_cast<const T*>(a.gate)[tok * a.ldg + h])));
+}
+
 // Four columns of a finished row: the sink joined, the sum divided out, the gate applied.
 template <typename T, int HD>
 __device__ __forceinline__ void finish_row(const AttnArgs& a, int64_t tok, int h, int col, float m, float l,
-                                           const float (&o)[4], float z, bool write_lse) {
+                                           const float (&o)[4], float z, float gate, bool write_lse) {
   float f = 1.f;
   if (a.k_sink != nullptr) {
     const float mt = fmaxf(m, z);
@@ -277,21 +290,41 @@ __device__ __forceinline__ void finish_row(const AttnArgs& a, int64_t tok, int h
     l = l * f + exp2f(z - mt);
     m = mt;
   }
-  float inv = l > 0.f ? f / l : (l != l ? l : 0.f);
-  if (a.gate != nullptr) inv *= 1.f / (1.f + expf(-to_f32(reinterpret_cast<const T*>(a.gate)[tok * a.ldg + h])));
+  const float inv = gate * (l > 0.f ? f / l : (l != l ? l : 0.f));
   const typename Pair<T>::type v[2] = {Pair<T>::from_f(o[0] * inv, o[1] * inv), Pair<T>::from_f(o[2] * inv, o[3] * inv)};
   *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.o) + (tok * a.H + h) * HD + col) =
       make_uint2(*reinterpret_cast<const uint32_t*>(&v[0]), *reinterpret_cast<const uint32_t*>(&v[1]));
   if (write_lse && a.lse != nullptr) a.lse[tok * a.H + h] = l > 0.f ? (m + log2f(l)) * 0.6931471805599453f : (l != l ? l : -INFINITY);
 }
 
+// The steps 0 .. all - 1 cut into nb runs, the first `more` of them one step longer.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  return (a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
+struct Runs {
+  int64_t nb, size, more;
+  __device__ __forceinline__ Runs(int64_t all, int blocks) {
+    nb = all < blocks ? all : blocks;
+    size = quotient(all, nb);
+    more = all - size * nb;
+  }
+  __device__ __forceinline__ int64_t begin(int64_t b) const { return b * size + min(b, more); }
+  __device__ __forceinline__ int64_t block_of(int64_t t) const {
+    const int64_t edge = more * (size + 1);
+    return t < edge ? quotient(t, size + 1) : more + quotient(t - edge, size);
+  }
+};
+
 template <typename T, int HD>
 __global__ void __launch_bounds__(160, 2)
     paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                        const AttnArgs a, float* parts, int64_t* counts) {
+                        const AttnArgs a, float* parts) {
   using L = DecSmem<HD>;
-  constexpr int ATOMS = HD / 64;
+  constexpr int ATOMS = HD / 64, TILE = L::TILE, OVER = L::OVER;
   constexpr int KS = HD / 16;              // k-steps of S
+  constexpr int KEYS = TILE / 4;           // keys of a warp
+  constexpr int NT = KEYS / 8;
+  constexpr int FEW = 512 / HD;            // rows that go out in one pass
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
@@ -305,6 +338,7 @@ __global__ void __launch_bounds__(160, 2)
   const int G = a.H / a.Hkv;
   const int blocks_g = (G + DEC_ROWS - 1) / DEC_ROWS;
   const int units = a.Hkv * blocks_g;      // per sequence
+  const int prows = part_rows(G);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < L::STAGES; ++s) {
@@ -314,11 +348,15 @@ __global__ void __launch_bounds__(160, 2)
     *s_abort = 0;
     fence_barrier_init();
   }
+  if (threadIdx.x == 128) {
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
   // Count the tiles: thread t those of a contiguous share of the sequences.
   const int per = (a.num_seqs + 159) / 160;
   const int q0 = min(a.num_seqs, (int)threadIdx.x * per), q1 = min(a.num_seqs, q0 + per);
   int64_t mine = 0;
-  for (int s = q0; s < q1; ++s) mine += span_of(a, s).tiles;
+  for (int s = q0; s < q1; ++s) mine += span_of<TILE>(a, s).tiles + OVER;
   int64_t inc = mine;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
@@ -333,15 +371,14 @@ __global__ void __launch_bounds__(160, 2)
     total += s_warp[w];
   }
   const int64_t all = total * units;
-  const int64_t nb = min((int64_t)gridDim.x, all);      // blocks with work
-  const int64_t begin = blockIdx.x * all / nb, end = (blockIdx.x + 1) * all / nb;
-  const bool works = blockIdx.x < nb;
+  const Runs runs(all, (int)gridDim.x);
+  const int64_t begin = runs.begin(blockIdx.x), end = runs.begin(blockIdx.x + 1);
+  const bool works = blockIdx.x < runs.nb;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the join waits for this grid's end itself
   {
     int64_t at = before;
     for (int s = q0; s < q1; ++s) {
-      const int n = span_of(a, s).tiles;
-      if (blockIdx.x == 0) counts[s] = at;
+      const int n = span_of<TILE>(a, s).tiles + OVER;
       if (works && begin >= at * units && begin < (at + n) * units) {
         *s_seq = s;
         s_run[1] = at;
@@ -349,56 +386,75 @@ __global__ void __launch_bounds__(160, 2)
       at += n;
     }
   }
-  if (blockIdx.x == 0 && threadIdx.x == 0) counts[a.num_seqs] = total;
   __syncthreads();
   if (!works) return;
 
-  int seq = *s_seq;
-  Span sp = span_of(a, seq);
-  int unit, tile;
+  // The run as parts: unit (seq, unit), its tiles [tile, tile + n).
+  int seq = *s_seq, unit, at;              // at: step of the unit, its first OVER steps are no tiles
+  Span sp = span_of<TILE>(a, seq);
   {
     const int64_t rest = begin - s_run[1] * units;
-    unit = (int)(rest / sp.tiles);
-    tile = (int)(rest - (int64_t)unit * sp.tiles);
+    unit = (int)quotient(rest, sp.tiles + OVER);
+    at = (int)(rest - (int64_t)unit * (sp.tiles + OVER));
   }
-  auto advance = [&]() {
-    if (++tile < sp.tiles) return;
-    tile = 0;
+  int64_t left = end - begin;
+  int tile = 0, n = 0;
+  auto advance_unit = [&]() {              // past a unit that is done (a run that ends in one stays)
+    if (at < sp.tiles + OVER) return;
+    at = 0;
     if (++unit < units) return;
     unit = 0;
-    ++seq;
-    if (seq < a.num_seqs) sp = span_of(a, seq);
+    if (++seq < a.num_seqs) sp = span_of<TILE>(a, seq);
+  };
+  // the next part with a tile in it; false at the end of the run
+  auto next_part = [&]() -> bool {
+    while (left > 0) {
+      const int steps = (int)min((int64_t)(sp.tiles + OVER - at), left);
+      tile = max(at - OVER, 0);
+      n = at + steps - OVER - tile;
+      left -= steps;
+      at += steps;
+      if (n > 0) return true;
+      advance_unit();
+    }
+    return false;
   };
 
   if (warp == 4) {
     // ---------------------------------------------------------------- loads
-    const int rows = min(a.page, DEC_TILE);            // rows per box
-    const int per_tile = DEC_TILE / rows;              // pages of a tile
+    const int rows = min(a.page, TILE);                // rows per box
+    const int per_tile = TILE / rows;                  // pages of a tile
     const int boxes = per_tile * ATOMS * 2;            // lane = (page, atom, K or V)
-    const int pg = lane / (2 * ATOMS), at = (lane >> 1) % ATOMS, kv = lane & 1;
+    const int pg = lane / (2 * ATOMS), atom = (lane >> 1) % ATOMS, kv = lane & 1;
     int it = 0;
     uint32_t issued = 0, par = 0;
-    for (int64_t g = begin; g < end; ++g, ++it) {
-      const int st = it % L::STAGES;
+    bool ok = true;
+    while (ok && next_part()) {
       const int hk = unit / blocks_g;
-      const int key = (sp.first_tile + tile) * DEC_TILE + pg * rows;
-      int page = (int)a.num_pages;                     // past the pool: TMA fills zeros
-      if (lane < boxes && key < sp.len && key + rows > sp.first_key) {
-        page = __ldg(a.block_table + seq * a.bt_ld + key / a.page);
-        if ((unsigned)page >= (unsigned)a.num_pages) {
-          record_error(ZS_DEVERR_INDEX);
-          page = (int)a.num_pages;
+      for (int j = 0; j < n; ++j, ++it) {
+        const int st = it % L::STAGES;
+        const int key = (sp.first_tile + tile + j) * TILE + pg * rows;
+        int page = (int)a.num_pages;                   // past the pool: TMA fills zeros
+        if (lane < boxes && key < sp.len && key + rows > sp.first_key) {
+          page = __ldg(a.block_table + seq * a.bt_ld + key / a.page);
+          if ((unsigned)page >= (unsigned)a.num_pages) {
+            record_error(ZS_DEVERR_INDEX);
+            page = (int)a.num_pages;
+          }
         }
+        if (!warp_wait(&empty[st], ((it / L::STAGES) & 1) ^ 1, s_abort, ZS_DEVERR_TIMEOUT_PRODUCER)) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) mbar_arrive_expect_tx(&full[st], L::STAGE);
+        __syncwarp();
+        if (lane < boxes)
+          tma_load_3d(smem + st * L::STAGE + kv * L::MAT + atom * (TILE * 128) + pg * rows * 128, kv ? &tmV : &tmK,
+                      &full[st], atom * 64, hk * a.page + key % a.page, page);
+        issued |= 1u << st;
+        par = (par & ~(1u << st)) | ((uint32_t)((it / L::STAGES) & 1) << st);
       }
-      if (!warp_wait(&empty[st], ((it / L::STAGES) & 1) ^ 1, s_abort, ZS_DEVERR_TIMEOUT_PRODUCER)) break;
-      if (lane == 0) mbar_arrive_expect_tx(&full[st], L::STAGE);
-      __syncwarp();
-      if (lane < boxes)
-        tma_load_3d(smem + st * L::STAGE + kv * L::MAT + at * (DEC_TILE * 128) + pg * rows * 128, kv ? &tmV : &tmK,
-                    &full[st], at * 64, hk * a.page + key % a.page, page);
-      issued |= 1u << st;
-      par = (par & ~(1u << st)) | ((uint32_t)((it / L::STAGES) & 1) << st);
-      advance();
+      advance_unit();
     }
     for (int s = 0; s < L::STAGES; ++s)                // copies in flight land before the warp leaves
       if (issued >> s & 1) mbar_wait(&full[s], par >> s & 1, nullptr, ZS_DEVERR_TIMEOUT_DRAIN);
@@ -413,27 +469,28 @@ __global__ void __launch_bounds__(160, 2)
   uint32_t qf[KS][4];
   float o[HD / 8][4];
   float m[2], l[2];
-  int it = 0, first = 1;                               // first: the part began with the block's run
-  int64_t g = begin;
-  while (g < end) {
-    // a part: tiles [tile, ...) of (seq, unit), to the unit's or the run's end
+  int it = 0;
+  bool first = true;                                   // the part begins with the block's run
+  while (next_part()) {
     const int hk = unit / blocks_g, g0 = (unit - hk * blocks_g) * DEC_ROWS;
     const int h0 = hk * G + g0, nrow = min(DEC_ROWS, G - g0);
-    const bool from_start = tile == 0;
-    const int64_t left = end - g;
-    const int n = (int)min((int64_t)(sp.tiles - tile), left);
-    const bool to_end = tile + n == sp.tiles;
-    const int pseq = seq;
+    const bool whole = n == sp.tiles;
     {
       const T* q = reinterpret_cast<const T*>(a.q) + (int64_t)seq * a.ldq + (int64_t)h0 * HD + c4 * 2;
 #pragma unroll
       for (int kk = 0; kk < KS; ++kk)
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const int row = r4 + (x & 1) * 8;
-          qf[kk][x] = row < nrow ? *reinterpret_cast<const uint32_t*>(q + row * HD + kk * 16 + (x >> 1) * 8) : 0u;
+          const int qr = r4 + (x & 1) * 8;
+          qf[kk][x] = qr < nrow ? *reinterpret_cast<const uint32_t*>(q + qr * HD + kk * 16 + (x >> 1) * 8) : 0u;
         }
     }
+    // asked for here, used when the part ends
+    const int mine = h0 + min((int)threadIdx.x / (nrow <= FEW ? HD / 4 : 8), nrow - 1);   // this thread's row going out
+    float z = 0.f;
+    if (whole && a.k_sink != nullptr)
+      z = nrow <= FEW ? sink_logit<T, HD, HD / 4>(a, seq, mine) : sink_logit<T, HD, 8>(a, seq, mine);
+    const float gate = whole ? gate_of<T>(a, seq, mine) : 1.f;
 #pragma unroll
     for (int c = 0; c < HD / 8; ++c)
 #pragma unroll
@@ -442,24 +499,29 @@ __global__ void __launch_bounds__(160, 2)
     l[0] = l[1] = 0.f;
     for (int j = 0; j < n; ++j, ++it) {
       const int st = it % L::STAGES;
-      const int key0 = (sp.first_tile + tile + j) * DEC_TILE + warp * 16;
+      const int key0 = (sp.first_tile + tile + j) * TILE + warp * KEYS;
       if (!warp_wait(&full[st], (it / L::STAGES) & 1, s_abort, ZS_DEVERR_TIMEOUT_EPILOGUE)) break;
       const uint32_t kb = smem_u32(smem + st * L::STAGE), vb = kb + L::MAT;
-      float s[2][4];
+      float s[NT][4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[0][e] = s[1][e] = 0.f;
-      const int krow = warp * 16 + (lane >> 4) * 8 + (lane & 7);
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[t][e] = 0.f;
 #pragma unroll
       for (int kk = 0; kk < KS; ++kk) {
         const int ch = kk * 2 + ((lane >> 3) & 1);     // 16-byte chunk of the row
-        uint32_t b[4];
-        ldsm_x4(kb + (ch >> 3) * (DEC_TILE * 128) + krow * 128 + (((ch & 7) ^ (krow & 7)) << 4), b);
-        mma_16816<T>(s[0], qf[kk], b[0], b[1]);
-        mma_16816<T>(s[1], qf[kk], b[2], b[3]);
-      }
-      const bool edge = key0 + 16 > sp.len || key0 < sp.first_key;
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < NT; t += 2) {
+          const int krow = warp * KEYS + t * 8 + (lane >> 4) * 8 + (lane & 7);
+          uint32_t b[4];
+          ldsm_x4(kb + (ch >> 3) * (TILE * 128) + krow * 128 + (((ch & 7) ^ (krow & 7)) << 4), b);
+          mma_16816<T>(s[t], qf[kk], b[0], b[1]);
+          mma_16816<T>(s[t + 1], qf[kk], b[2], b[3]);
+        }
+      }
+      const bool edge = key0 + KEYS > sp.len || key0 < sp.first_key;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           s[t][e] *= a.scale_log2;
@@ -474,7 +536,9 @@ __global__ void __launch_bounds__(160, 2)
       bool grow = false;
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        float mx = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
+        float mx = fmaxf(s[0][2 * r], s[0][2 * r + 1]);
+#pragma unroll
+        for (int t = 1; t < NT; ++t) mx = fmaxf(mx, fmaxf(s[t][2 * r], s[t][2 * r + 1]));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
         f[r] = 1.f;
@@ -495,40 +559,43 @@ __global__ void __launch_bounds__(160, 2)
         }
       }
       // P in the cache's type for the second product, its sum in f32 before the rounding
-      uint32_t p[4];
+      uint32_t p[NT / 2][4];
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const float mu = m[r] == -INFINITY ? 0.f : m[r];
           const float e0 = attn::fast_exp2(s[t][2 * r] - mu), e1 = attn::fast_exp2(s[t][2 * r + 1] - mu);
           l[r] += e0 + e1;
           const typename Pair<T>::type pp = Pair<T>::from_f(e0, e1);
-          p[t * 2 + r] = *reinterpret_cast<const uint32_t*>(&pp);
+          p[t / 2][(t & 1) * 2 + r] = *reinterpret_cast<const uint32_t*>(&pp);
         }
-      const int vrow = warp * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
-      uint32_t keep[2] = {0xffffffffu, 0xffffffffu};   // values of keys that are not seen count as zero
-      if (edge) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const int k = key0 + t * 8 + c4 * 2;
-          keep[t] = (k < sp.len && k >= sp.first_key ? 0xffffu : 0u) |
-                    (k + 1 < sp.len && k + 1 >= sp.first_key ? 0xffff0000u : 0u);
-        }
-      }
-#pragma unroll
-      for (int c = 0; c < HD / 8; c += 2) {
-        const int ch = c + (lane >> 4);
-        uint32_t b[4];
-        ldsm_x4_t(vb + (ch >> 3) * (DEC_TILE * 128) + vrow * 128 + (((ch & 7) ^ (vrow & 7)) << 4), b);
+      for (int ks = 0; ks < NT / 2; ++ks) {
+        const int vrow = warp * KEYS + ks * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
+        uint32_t keep[2] = {0xffffffffu, 0xffffffffu};   // values of keys that are not seen count as zero
         if (edge) {
-          b[0] &= keep[0];
-          b[1] &= keep[1];
-          b[2] &= keep[0];
-          b[3] &= keep[1];
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const int k = key0 + ks * 16 + t * 8 + c4 * 2;
+            keep[t] = (k < sp.len && k >= sp.first_key ? 0xffffu : 0u) |
+                      (k + 1 < sp.len && k + 1 >= sp.first_key ? 0xffff0000u : 0u);
+          }
         }
-        mma_16816<T>(o[c], p, b[0], b[1]);
-        mma_16816<T>(o[c + 1], p, b[2], b[3]);
+#pragma unroll
+        for (int c = 0; c < HD / 8; c += 2) {
+          const int ch = c + (lane >> 4);
+          uint32_t b[4];
+          ldsm_x4_t(vb + (ch >> 3) * (TILE * 128) + vrow * 128 + (((ch & 7) ^ (vrow & 7)) << 4), b);
+          if (edge) {
+            b[0] &= keep[0];
+            b[1] &= keep[1];
+            b[2] &= keep[0];
+            b[3] &= keep[1];
+          }
+          mma_16816<T>(o[c], p[ks], b[0], b[1]);
+          mma_16816<T>(o[c + 1], p[ks], b[2], b[3]);
+        }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[st]);
@@ -543,50 +610,53 @@ __global__ void __launch_bounds__(160, 2)
         s_l[warp * DEC_ROWS + r4 + r * 8] = l[r];
       }
     }
-    const bool whole = from_start && to_end;
-    const int row = threadIdx.x >> 3, col = (threadIdx.x & 7) * 4;
-    const int h = h0 + min(row, nrow - 1);
-    const float z = whole && a.k_sink != nullptr ? sink_logit<T, HD, 8>(a, pseq, h) : 0.f;
-    float* part = parts + ((int64_t)blockIdx.x * 2 + (first ? 0 : 1)) * part_floats(HD);
+    float* part = parts + ((int64_t)blockIdx.x * 2 + (first ? 0 : 1)) * part_floats(HD, prows);
+    // COLS columns at a time through the buffer [4 warps][rows][COLS]: a group of few heads goes
+    // out in one pass, 16 in HD / 32
     bool stop = false;
+    auto emit = [&](auto cols) {
+      constexpr int COLS = decltype(cols)::value, ROWS = 512 / COLS, LD = COLS + 8;
+      const int row = threadIdx.x / (COLS / 4), col = threadIdx.x % (COLS / 4) * 4;
 #pragma unroll
-    for (int ps = 0; ps < HD / 32; ++ps) {             // 32 columns at a time
+      for (int ps = 0; ps < HD / COLS; ++ps) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        float* dst = s_o + (warp * DEC_ROWS + r4) * DEC_LDO + c * 8 + c4 * 2;
-        *reinterpret_cast<float2*>(dst) = make_float2(o[ps * 4 + c][0], o[ps * 4 + c][1]);
-        *reinterpret_cast<float2*>(dst + 8 * DEC_LDO) = make_float2(o[ps * 4 + c][2], o[ps * 4 + c][3]);
-      }
-      consumer_any(false);
-      float mt = -INFINITY, lt = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int w = 0; w < 4; ++w) mt = fmaxf(mt, s_m[w * DEC_ROWS + row]);
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float mw = s_m[w * DEC_ROWS + row];
-        const float fw = mw == -INFINITY ? 0.f : exp2f(mw - mt);
-        lt = fmaf(fw, s_l[w * DEC_ROWS + row], lt);
-        const float4 x = *reinterpret_cast<const float4*>(s_o + (w * DEC_ROWS + row) * DEC_LDO + col);
-        acc[0] = fmaf(fw, x.x, acc[0]);
-        acc[1] = fmaf(fw, x.y, acc[1]);
-        acc[2] = fmaf(fw, x.z, acc[2]);
-        acc[3] = fmaf(fw, x.w, acc[3]);
-      }
-      if (row < nrow) {
-        if (whole) {
-          finish_row<T, HD>(a, pseq, h, ps * 32 + col, mt, lt, acc, z, ps == 0 && col == 0);
-        } else {
-          *reinterpret_cast<float4*>(part + row * HD + ps * 32 + col) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-          if (ps == 0 && col == 0) *reinterpret_cast<float2*>(part + DEC_ROWS * HD + row * 2) = make_float2(mt, lt);
+        for (int c = 0; c < COLS / 8; ++c) {
+          const float(&oc)[4] = o[ps * (COLS / 8) + c];
+          float* dst = s_o + (warp * ROWS + r4) * LD + c * 8 + c4 * 2;
+          if (ROWS >= 8 || r4 < ROWS) *reinterpret_cast<float2*>(dst) = make_float2(oc[0], oc[1]);
+          if (ROWS > 8) *reinterpret_cast<float2*>(dst + 8 * LD) = make_float2(oc[2], oc[3]);
         }
+        consumer_any(false);
+        float mt = -INFINITY, lt = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) mt = fmaxf(mt, s_m[w * DEC_ROWS + row]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float mw = s_m[w * DEC_ROWS + row];
+          const float fw = mw == -INFINITY ? 0.f : exp2f(mw - mt);
+          lt = fmaf(fw, s_l[w * DEC_ROWS + row], lt);
+          const float4 x = *reinterpret_cast<const float4*>(s_o + (w * ROWS + row) * LD + col);
+          acc[0] = fmaf(fw, x.x, acc[0]);
+          acc[1] = fmaf(fw, x.y, acc[1]);
+          acc[2] = fmaf(fw, x.z, acc[2]);
+          acc[3] = fmaf(fw, x.w, acc[3]);
+        }
+        if (row < nrow) {
+          if (whole) {
+            finish_row<T, HD>(a, seq, h0 + row, ps * COLS + col, mt, lt, acc, z, gate, ps == 0 && col == 0);
+          } else {
+            *reinterpret_cast<float4*>(part + row * HD + ps * COLS + col) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+            if (ps == 0 && col == 0) *reinterpret_cast<float2*>(part + prows * HD + row * 2) = make_float2(mt, lt);
+          }
+        }
+        stop = consumer_any(*s_abort);                 // also: the buffer may be written again
       }
-      stop = consumer_any(*s_abort);                   // also: the buffer may be written again
-    }
+    };
+    if (nrow <= FEW) emit(std::integral_constant<int, HD>());
+    else emit(std::integral_constant<int, 32>());
     if (stop) return;
-    g += n;
-    tile += n - 1;
-    advance();
-    first = 0;
+    advance_unit();
+    first = false;
   }
 }
 
@@ -597,26 +667,49 @@ constexpr int JOIN_WARPS = 8;
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const AttnArgs a, const float* parts,
-                                                                     const int64_t* counts, int decode_blocks) {
+                                                                     int decode_blocks) {
   constexpr int SUB = 128 / HD;            // parts side by side in a warp
+  constexpr int OVER = DecSmem<HD>::OVER, TILE = DecSmem<HD>::TILE;
   __shared__ float s_o[JOIN_WARPS][HD], s_ml[JOIN_WARPS][2];
+  __shared__ int64_t s_n[JOIN_WARPS][2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = a.H / a.Hkv;
   const int blocks_g = (G + DEC_ROWS - 1) / DEC_ROWS;
-  const int units = a.Hkv * blocks_g;
+  const int units = a.Hkv * blocks_g, prows = part_rows(G);
   const int seq = blockIdx.x, unit = blockIdx.y;
   const int hk = unit / blocks_g, g0 = (unit - hk * blocks_g) * DEC_ROWS;
   const int h0 = hk * G + g0, nrow = min(DEC_ROWS, G - g0);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int64_t before = counts[seq], tiles = counts[seq + 1] - before;
-  const int64_t all = counts[a.num_seqs] * units, nb = min((int64_t)decode_blocks, all);
-  const int64_t t0 = before * units + unit * tiles, t1 = t0 + tiles - 1;
-  // block of tile t: the last b with floor(b * all / nb) <= t
-  const int b0 = (int)(((t0 + 1) * nb - 1) / all), b1 = (int)(((t1 + 1) * nb - 1) / all);
+  // all that does not come from the decode kernel, before its end
+  int64_t before = 0, total = 0;
+  for (int s = threadIdx.x; s < a.num_seqs; s += JOIN_WARPS * 32) {
+    const int n = span_of<TILE>(a, s).tiles + OVER;
+    total += n;
+    if (s < seq) before += n;
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    before += __shfl_xor_sync(0xffffffffu, before, off);
+    total += __shfl_xor_sync(0xffffffffu, total, off);
+  }
+  if (lane == 0) {
+    s_n[warp][0] = before;
+    s_n[warp][1] = total;
+  }
+  const int steps = span_of<TILE>(a, seq).tiles + OVER;
+  __syncthreads();
+  before = total = 0;
+#pragma unroll
+  for (int w = 0; w < JOIN_WARPS; ++w) {
+    before += s_n[w][0];
+    total += s_n[w][1];
+  }
+  const Runs runs(total * units, decode_blocks);
+  const int64_t t0 = before * units + (int64_t)unit * steps + OVER, t1 = t0 + steps - OVER - 1;   // its first and last tile
+  const int b0 = (int)runs.block_of(t0), b1 = (int)runs.block_of(t1);
   if (b0 == b1) return;
-  // a block's first part lies in its slot 0; one that starts inside the block's run (only the
-  // first can) in slot 1
-  const int shift = b0 * all / nb < t0 ? 1 : 0;
+  // a block's first part lies in its slot 0; the first block's part may come after another one
+  const int shift = runs.begin(b0) < t0 - OVER ? 1 : 0;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int shares = nrow >= JOIN_WARPS ? 1 : JOIN_WARPS / nrow;
   const int share = warp % shares, sub = lane / (HD / 4), col = (lane % (HD / 4)) * 4;
   for (int row = warp / shares; row < nrow; row += JOIN_WARPS / shares) {
@@ -631,8 +724,8 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const AttnA
         ml[e] = make_float2(-INFINITY, 0.f);
         o[e] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (bb <= b1) {
-          const float* part = parts + ((int64_t)bb * 2 + (bb == b0 ? shift : 0)) * part_floats(HD);
-          ml[e] = *reinterpret_cast<const float2*>(part + DEC_ROWS * HD + row * 2);
+          const float* part = parts + ((int64_t)bb * 2 + (bb == b0 ? shift : 0)) * part_floats(HD, prows);
+          ml[e] = *reinterpret_cast<const float2*>(part + prows * HD + row * 2);
           o[e] = *reinterpret_cast<const float4*>(part + row * HD + col);
         }
       }
@@ -666,7 +759,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const AttnA
     } else {
       const int h = h0 + row;
       const float z = a.k_sink != nullptr ? sink_logit<T, HD, 32>(a, seq, h) : 0.f;
-      if (sub == 0) finish_row<T, HD>(a, seq, h, col, m, l, acc, z, col == 0);
+      if (sub == 0) finish_row<T, HD>(a, seq, h, col, m, l, acc, z, gate_of<T>(a, seq, h), col == 0);
     }
   }
   if (shares == 1) return;
@@ -683,7 +776,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const AttnA
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[e] = fmaf(f, s_o[w][col + e], acc[e]);
   }
-  if (sub == 0) finish_row<T, HD>(a, seq, h, col, m, l, acc, z, col == 0);
+  if (sub == 0) finish_row<T, HD>(a, seq, h, col, m, l, acc, z, gate_of<T>(a, seq, h), col == 0);
 }
 
 }  // namespace paged
@@ -768,32 +861,30 @@ template <typename T, int HD>
 static int launch_decode(const paged::AttnArgs& a, int dtype, void* workspace, cudaStream_t stream) {
   using L = paged::DecSmem<HD>;
   CUtensorMap tk, tv;
-  const int box = a.page < paged::DEC_TILE ? a.page : paged::DEC_TILE;
+  const int box = a.page < L::TILE ? a.page : L::TILE;
   int rc = make_page_tmap(&tk, a.k_pages, dtype, HD, (int64_t)a.Hkv * a.page, a.num_pages, a.page_stride, box);
   if (rc != ZS_OK) return rc;
   rc = make_page_tmap(&tv, a.v_pages, dtype, HD, (int64_t)a.Hkv * a.page, a.num_pages, a.page_stride, box);
   if (rc != ZS_OK) return rc;
   // no more blocks than tiles that the table (or the window) leaves room for
   const int G = a.H / a.Hkv, units = a.Hkv * ((G + paged::DEC_ROWS - 1) / paged::DEC_ROWS);
-  int64_t most = ((int64_t)a.max_pages * a.page + paged::DEC_TILE - 1) / paged::DEC_TILE;
-  if (a.window > 0) most = min(most, (int64_t)(a.window + paged::DEC_TILE - 2) / paged::DEC_TILE + 1);
-  const int64_t all = most * a.num_seqs * units;
+  int64_t most = ((int64_t)a.max_pages * a.page + L::TILE - 1) / L::TILE;
+  if (a.window > 0) most = min(most, ((int64_t)a.window + L::TILE - 2) / L::TILE + 1);
+  const int64_t all = (most + L::OVER) * a.num_seqs * units;
   const int resident = 2 * num_sms() < paged::DEC_MAX_BLOCKS ? 2 * num_sms() : paged::DEC_MAX_BLOCKS;
   const int blocks = (int)(all < resident ? all : resident);
-  int64_t* counts = reinterpret_cast<int64_t*>((reinterpret_cast<uintptr_t>(workspace) + 15) & ~uintptr_t(15));
-  float* parts = reinterpret_cast<float*>(counts + ((a.num_seqs + 2) & ~1));
+  float* parts = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(workspace) + 15) & ~uintptr_t(15));
   ZS_CUDA_TRY(cudaFuncSetAttribute(paged::paged_decode_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::ALLOC));
-  paged::paged_decode_kernel<T, HD><<<blocks, 160, L::ALLOC, stream>>>(tk, tv, a, parts, counts);
+  paged::paged_decode_kernel<T, HD><<<blocks, 160, L::ALLOC, stream>>>(tk, tv, a, parts);
   ZS_CUDA_TRY(cudaGetLastError());
   if (most == 1) return ZS_OK;                         // nothing can be split
   return launch_after(paged::paged_join_kernel<T, HD>, dim3((unsigned)a.num_seqs, (unsigned)units),
-                      dim3(paged::JOIN_WARPS * 32), stream, a, parts, counts, blocks);
+                      dim3(paged::JOIN_WARPS * 32), stream, a, parts, blocks);
 }
 
 extern "C" size_t zs_paged_decode_workspace(int num_seqs, int H, int Hkv, int hd) {
-  (void)H, (void)Hkv;
-  if (num_seqs < 0 || hd < 0) return 0;
-  return (size_t)((num_seqs + 4) * 8 + paged::DEC_MAX_BLOCKS * 2 * paged::part_floats(hd) * 4 + 64);
+  if (num_seqs < 0 || hd < 0 || Hkv < 1) return 0;
+  return (size_t)(paged::DEC_MAX_BLOCKS * 2 * paged::part_floats(hd, paged::part_rows(H / Hkv)) * 4 + 64);
 }
 
 extern "C" int zs_paged_decode_attention(const void* q, int64_t ldq, const void* k_pages, const void* v_pages,
