@@ -153,8 +153,8 @@ __global__ void __launch_bounds__(256, 3) paged_append_kernel(const AppendArgs a
   int page = -1;
   bool live = pos >= 0;                // no sequence or a negative position: zero q, nothing stored
   if (live) {
-    const int pi = (int)pos / a.page;  // positions lie below 2^31
-    if (pi < a.max_pages && (a.rot == 0 || pos < a.table_rows)) page = __ldg(a.block_table + seq * a.bt_ld + pi);
+    if (pos < (int64_t)a.max_pages * a.page && (a.rot == 0 || pos < a.table_rows))   // below 2^31
+      page = __ldg(a.block_table + seq * a.bt_ld + (int)pos / a.page);
     if (page < 0 || page >= a.num_pages) {
       if (lane == 0 && part == 0) record_error(ZS_DEVERR_INDEX);
       live = false;

@@ -38,95 +38,11 @@ struct AttnArgs {
   float* lse;                  // nullable [tokens, H]
 };
 
-__device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i) {
-  if (dtype == ZS_F32) return reinterpret_cast<const float*>(p)[i];
-  if (dtype == ZS_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
-  return __half2float(reinterpret_cast<const __half*>(p)[i]);
-}
-
 // A sequence's length, no longer than its row of the block table.
 __device__ __forceinline__ int cut_length(const AttnArgs& a, int seq) {
   const int len = __ldg(a.seq_lens + seq), cap = a.max_pages * a.page;
   if (len > cap) record_error(ZS_DEVERR_INDEX);
   return len > cap ? cap : len;
-}
-
-// Plain form: one block per (token, head), four warps over the keys, an online
-// softmax per warp, joined at the end.
-template <typename T, int HD>
-__global__ void __launch_bounds__(128) paged_attn_kernel(const AttnArgs a) {
-  constexpr int E = HD / 32;
-  __shared__ float s_m[4], s_l[4], s_o[4][HD];
-  const int64_t tok = blockIdx.x;
-  const int h = blockIdx.y, hk = h / (a.H / a.Hkv);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int seq = (int)tok;
-  int64_t pos;
-  if (a.cu != nullptr) {
-    seq = sequence_of(a.cu, a.num_seqs, (int)tok);
-    if (seq < 0) {                     // a row of no sequence: zero
-      for (int e = threadIdx.x; e < HD; e += 128) reinterpret_cast<T*>(a.o)[(tok * a.H + h) * HD + e] = from_f32<T>(0.f);
-      if (a.lse != nullptr && threadIdx.x == 0) a.lse[tok * a.H + h] = -INFINITY;
-      return;
-    }
-    pos = (int64_t)cut_length(a, seq) - a.cu[seq + 1] + tok;
-  } else {
-    pos = (int64_t)cut_length(a, seq) - 1;
-  }
-  const T* q = reinterpret_cast<const T*>(a.q) + tok * a.ldq + (int64_t)h * HD;
-  float qv[E], ov[E];
-  float m = -INFINITY, l = 0.f;
-  for (int e = 0; e < E; ++e) {
-    qv[e] = to_f32(q[lane * E + e]);
-    ov[e] = 0.f;
-  }
-  if (a.k_sink != nullptr && warp == 0) {
-    float dot = 0.f;
-    for (int e = 0; e < E; ++e) dot = fmaf(qv[e], load_any(a.k_sink, a.sink_dtype, (int64_t)h * HD + lane * E + e), dot);
-    for (int off = 16; off > 0; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
-    m = dot * a.scale;
-    l = 1.f;
-  }
-  const int64_t first = a.window > 0 && pos - a.window + 1 > 0 ? pos - a.window + 1 : 0;
-  for (int64_t k = first + warp; k <= pos; k += 4) {
-    const int pg = a.block_table[seq * a.bt_ld + k / a.page];
-    if (pg < 0 || pg >= a.num_pages) {
-      if (lane == 0) record_error(ZS_DEVERR_INDEX);
-    }
-    const bool ok = pg >= 0 && pg < a.num_pages;
-    const int64_t at = (ok ? pg : 0) * a.page_stride + ((int64_t)hk * a.page + k % a.page) * HD + lane * E;
-    float dot = 0.f;
-    for (int e = 0; e < E; ++e)
-      dot = fmaf(qv[e], ok ? to_f32(reinterpret_cast<const T*>(a.k_pages)[at + e]) : 0.f, dot);
-    for (int off = 16; off > 0; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
-    const float s = dot * a.scale, mn = fmaxf(m, s);
-    const float f = m == -INFINITY ? 0.f : expf(m - mn), p = expf(s - mn);
-    l = l * f + p;
-    for (int e = 0; e < E; ++e)
-      ov[e] = ov[e] * f + p * (ok ? to_f32(reinterpret_cast<const T*>(a.v_pages)[at + e]) : 0.f);
-    m = mn;
-  }
-  for (int e = 0; e < E; ++e) s_o[warp][lane * E + e] = ov[e];
-  if (lane == 0) {
-    s_m[warp] = m;
-    s_l[warp] = l;
-  }
-  __syncthreads();
-  if (threadIdx.x < HD) {
-    float mx = -INFINITY;
-    for (int w = 0; w < 4; ++w) mx = fmaxf(mx, s_m[w]);
-    float lt = 0.f, o = 0.f;
-    for (int w = 0; w < 4; ++w) {
-      const float f = s_m[w] == -INFINITY ? 0.f : expf(s_m[w] - mx);
-      lt += f * s_l[w];
-      o += f * s_o[w][threadIdx.x];
-    }
-    float inv = lt > 0.f ? 1.f / lt : 0.f;
-    if (a.gate != nullptr)
-      inv *= 1.f / (1.f + expf(-to_f32(reinterpret_cast<const T*>(a.gate)[tok * a.ldg + h])));
-    reinterpret_cast<T*>(a.o)[(tok * a.H + h) * HD + threadIdx.x] = from_f32<T>(o * inv);
-    if (a.lse != nullptr && threadIdx.x == 0) a.lse[tok * a.H + h] = lt > 0.f ? mx + logf(lt) : -INFINITY;
-  }
 }
 
 // ------------------------------------------------------------------------ decode
@@ -779,6 +695,558 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const AttnA
   if (sub == 0) finish_row<T, HD>(a, seq, h, col, m, l, acc, z, gate_of<T>(a, seq, h), col == 0);
 }
 
+// ------------------------------------------------------------------------ prompt
+//
+// Packed new tokens on the 5th-generation tensor cores.  The query heads of one key head share
+// its keys, so a row is a (token, head of the group) pair: a tile of 128 rows is 128 / G tokens
+// (short chunks after long prefixes fill it too), and a block is two such tiles of one
+// sequence and key head.  Blocks are numbered over all sequences from cu_seqlens on the device and
+// dealt to one persistent CTA per SM, last blocks (which see most keys) first; the loads of the
+// next block run while the rows of the last one go out.
+//
+//   warp 0      TMA: both Q tiles, then K and V of 128 keys, page by page, into a ring of slots
+//   warp 1      MMA: per key tile and query tile t, O_t += P_t V (P from tensor memory, the first
+//               half of its keys as soon as that half is there), then S_t = Q_t K^T
+//   warps 4..7  softmax of query tile 0, warps 8..11 of query tile 1: one row per thread; S from
+//               tensor memory, running max (log2 units, raised when it grows by more than 2^8)
+//               and sum, P in the cache's type over S's first 64 columns, at the end the row out
+// TMEM columns: S_t / P_t at t * 128, O_t at 256 + t * hd.
+
+constexpr int PT_ROWS = 128;              // rows of a query tile
+constexpr int PT_KEYS = 128;              // keys of a key tile
+constexpr int PT_THREADS = 384;
+// Registers: launched with 168 a thread (384 * 168 = 64512); the first four warps give back what
+// the softmax warps, which hold a whole row of S, take: 128 * (104 + 2 * 200) = 64512.
+constexpr int PT_REGS_AUX = 104, PT_REGS_SOFTMAX = 200;
+constexpr int PT_SUMS = 256;              // sequence groups whose block counts lie in shared memory
+
+template <int HD>
+struct PromptSmem {
+  static constexpr int TILE = 128 * HD * 2;
+  static constexpr int SLOTS = HD == 128 ? 5 : 8;
+  static constexpr int OFF_Q = 0;
+  static constexpr int OFF_KV = 2 * TILE;
+  static constexpr int OFF_SUMS = OFF_KV + SLOTS * TILE;
+  static constexpr int OFF_BAR = OFF_SUMS + (PT_SUMS + 8) * 4;
+  // q_full[2], q_empty[2], kv_full[SLOTS], kv_empty[SLOTS], s_full[2], p_half[2], p_full[2], o_done[2], o_free[2], done
+  static constexpr int NBAR = 4 + 2 * SLOTS + 11;
+  static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
+  static constexpr int TOTAL = OFF_MISC + 16;
+  static constexpr int ALLOC = TOTAL + 1024;
+};
+
+struct PromptBlock {
+  int seq, hk;
+  int tok0;                // packed row of the block's first token
+  int left;                // tokens of the sequence from there on
+  int pos0;                // position of the first token
+  int len;                 // tokens in the cache (cut)
+  int floor;               // no query of the sequence sees a key before this one
+  int lo[2], cnt[2];       // key tiles of the two query tiles
+};
+
+// Packed row i of cu_seqlens, inside the rows there are.
+__device__ __forceinline__ int cut_row(const AttnArgs& a, int i) {
+  return min(max(__ldg(a.cu + i), 0), (int)a.tokens);
+}
+// Blocks of a sequence.
+__device__ __forceinline__ int blocks_of(const AttnArgs& a, int seq, int per) {
+  const int n = cut_row(a, seq + 1) - cut_row(a, seq);
+  return n > 0 ? (n + per - 1) / per : 0;
+}
+
+// Block idx of the numbering (a warp asks together); sums[g]: blocks before sequence g * group.
+__device__ __forceinline__ PromptBlock find_block(const AttnArgs& a, const int* sums, int group, int per, int tpt,
+                                                  int64_t idx) {
+  const int lane = threadIdx.x & 31;
+  PromptBlock b;
+  const int blk = (int)(idx / a.Hkv);
+  b.hk = (int)(idx - (int64_t)blk * a.Hkv);
+  int lo = 0;
+#pragma unroll
+  for (int step = PT_SUMS / 32; step >= 1; step = step == 1 ? 0 : 1) {
+    const uint32_t below = __ballot_sync(0xffffffffu, (step > 1 || lane < PT_SUMS / 32) && sums[lo + lane * step] <= blk);
+    lo += (31 - __clz(below)) * step;
+  }
+  // the last of the group's sequences whose first block is not behind blk
+  int seq = lo * group, at = sums[lo];
+  for (int n; seq + 1 < a.num_seqs && blk >= at + (n = blocks_of(a, seq, per)); ++seq) at += n;
+  b.seq = seq;
+  const int first = cut_row(a, seq), n = cut_row(a, seq + 1) - first;
+  const int skip = (blk - at) * per;
+  b.tok0 = first + skip;
+  b.left = n - skip;
+  b.len = cut_length(a, seq);
+  b.pos0 = b.len - n + skip;
+  b.floor = a.window > 0 ? max(b.len - n - (a.window - 1), 0) : 0;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int rows = min(b.left - t * tpt, tpt);         // tokens of the tile
+    const int p0 = b.pos0 + t * tpt, p1 = p0 + rows - 1;
+    b.lo[t] = (a.window > 0 ? max(p0 - (a.window - 1), 0) : 0) / PT_KEYS;
+    b.cnt[t] = rows > 0 && p1 >= 0 ? p1 / PT_KEYS - b.lo[t] + 1 : 0;
+  }
+  return b;
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(PT_THREADS, 1)
+    paged_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                        const __grid_constant__ CUtensorMap tmV, const AttnArgs a) {
+  using L = PromptSmem<HD>;
+  constexpr int SLOTS = L::SLOTS;
+  constexpr int ATOMS = HD / 64, ATOM = 128 * 128;       // 128 rows of 128 bytes
+  constexpr uint32_t FMT = std::is_same<T, __half>::value ? 0 : 1;
+  constexpr uint32_t IDESC_S = idesc_f16(128, 128, FMT, 0, 0);
+  constexpr uint32_t IDESC_PV = idesc_f16(128, HD, FMT, 0, 1);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  int* sums = reinterpret_cast<int*>(smem + L::OFF_SUMS);
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
+  uint64_t* q_empty = q_full + 2;
+  uint64_t* kv_full = q_empty + 2;
+  uint64_t* kv_empty = kv_full + SLOTS;
+  uint64_t* s_full = kv_empty + SLOTS;
+  uint64_t* p_half = s_full + 2;
+  uint64_t* p_full = p_half + 2;
+  uint64_t* o_done = p_full + 2;
+  uint64_t* o_free = o_done + 2;
+  uint64_t* done = o_free + 2;
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
+  volatile int* s_abort = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 4);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int G = a.H / a.Hkv;
+  const int tpt = PT_ROWS / G, per = 2 * tpt;            // tokens of a tile, of a block
+
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&q_full[t], 1);
+      mbar_init(&q_empty[t], 5);                         // its last product, and the softmax warps
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_half[t], 4);
+      mbar_init(&p_full[t], 4);
+      mbar_init(&o_done[t], 1);
+      mbar_init(&o_free[t], 4);
+    }
+    for (int s = 0; s < SLOTS; ++s) {
+      mbar_init(&kv_full[s], 1);
+      mbar_init(&kv_empty[s], 2);                        // one release per query tile
+    }
+    mbar_init(done, 1);
+    *s_abort = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(s_tmem, 512);
+    tmem_relinquish();
+  }
+  // blocks before each group of sequences
+  const int group = (a.num_seqs + PT_SUMS - 1) / PT_SUMS;
+  if (warp >= 4) {                                       // 256 threads, one group each
+    const int g = threadIdx.x - 128;
+    int mine = 0;
+    for (int s = g * group; s < min(a.num_seqs, (g + 1) * group); ++s) mine += blocks_of(a, s, per);
+    int inc = mine;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, inc, off);
+      if (lane >= off) inc += o;
+    }
+    if (lane == 31) sums[PT_SUMS + warp - 4] = inc;
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    int before = inc - mine;
+    for (int w = 0; w < warp - 4; ++w) before += sums[PT_SUMS + w];
+    sums[g] = before;
+    if (g == PT_SUMS - 1) s_tmem[2] = before + mine;     // blocks of one key head
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *s_tmem;
+  const int64_t total = (int64_t)(int)s_tmem[2] * a.Hkv;
+  // all roles walk the same blocks
+#define ZS_EACH_BLOCK(i) for (int64_t i = total - 1 - (int64_t)blockIdx.x; i >= 0; i -= gridDim.x)
+
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PT_REGS_AUX));
+  if (warp == 0) {
+    // ------------------------------------------------------------------ loads
+    const int rows = min(a.page, PT_KEYS), boxes = PT_KEYS / rows * ATOMS;   // lane = (page, atom)
+    const int pg = lane / ATOMS, atom = lane % ATOMS;
+    uint32_t issued = 0, par = 0, q_n[2] = {0, 0};
+    int item = 0;
+    bool ok = true;
+    ZS_EACH_BLOCK(i) {
+      if (!ok) break;
+      const PromptBlock b = find_block(a, sums, group, per, tpt, i);
+      for (int t = 0; t < 2 && ok; ++t) {
+        if (b.cnt[t] == 0) continue;
+        ok = warp_wait(&q_empty[t], (q_n[t] & 1) ^ 1, s_abort, ZS_DEVERR_TIMEOUT_PRODUCER);
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&q_full[t], G * tpt * HD * 2);
+#pragma unroll
+          for (int at = 0; at < ATOMS; ++at)
+            tma_load_3d(smem + L::OFF_Q + t * L::TILE + at * ATOM, &tmQ, &q_full[t], at * 64, b.hk * G,
+                        b.tok0 + t * tpt);
+        }
+        ++q_n[t];
+      }
+      const int ulo = b.cnt[0] > 0 ? b.lo[0] : b.lo[1];
+      const int uhi = max(b.cnt[0] > 0 ? b.lo[0] + b.cnt[0] - 1 : 0, b.cnt[1] > 0 ? b.lo[1] + b.cnt[1] - 1 : 0);
+      if (b.cnt[0] + b.cnt[1] == 0) continue;
+      for (int j = ulo; ok && j <= uhi; ++j) {
+        if (!(j >= b.lo[0] && j < b.lo[0] + b.cnt[0]) && !(j >= b.lo[1] && j < b.lo[1] + b.cnt[1])) continue;
+        const int key = j * PT_KEYS + pg * rows;
+        int page = (int)a.num_pages;                     // past the pool: TMA fills zeros
+        if (lane < boxes && key < b.len && key + rows > b.floor) {
+          page = __ldg(a.block_table + b.seq * a.bt_ld + key / a.page);
+          if ((unsigned)page >= (unsigned)a.num_pages) {
+            record_error(ZS_DEVERR_INDEX);
+            page = (int)a.num_pages;
+          }
+        }
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv, ++item) {
+          const int st = item % SLOTS;
+          if (!warp_wait(&kv_empty[st], ((item / SLOTS) & 1) ^ 1, s_abort, ZS_DEVERR_TIMEOUT_PRODUCER)) {
+            ok = false;
+            break;
+          }
+          if (lane == 0) mbar_arrive_expect_tx(&kv_full[st], L::TILE);
+          __syncwarp();
+          if (lane < boxes)
+            tma_load_3d(smem + L::OFF_KV + st * L::TILE + atom * ATOM + pg * rows * 128, kv ? &tmV : &tmK, &kv_full[st],
+                        atom * 64, b.hk * a.page + key % a.page, page);
+          issued |= 1u << st;
+          par = (par & ~(1u << st)) | ((uint32_t)((item / SLOTS) & 1) << st);
+        }
+      }
+    }
+    // copies in flight land before the CTA leaves
+    for (int t = 0; t < 2; ++t)
+      if (q_n[t] > 0) mbar_wait(&q_full[t], (q_n[t] - 1) & 1, nullptr, ZS_DEVERR_TIMEOUT_DRAIN);
+    for (int s = 0; s < SLOTS; ++s)
+      if (issued & (1u << s)) mbar_wait(&kv_full[s], (par >> s) & 1, nullptr, ZS_DEVERR_TIMEOUT_DRAIN);
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ products
+    bool ok = true, issued_any = false;
+    int item = 0;
+    uint32_t q_n[2] = {0, 0};    // Q tiles waited for
+    uint32_t p_n[2] = {0, 0};    // P tiles waited for
+    uint32_t b_n[2] = {0, 0};    // blocks begun, per query tile
+    ZS_EACH_BLOCK(i) {
+      if (!ok) break;
+      const PromptBlock b = find_block(a, sums, group, per, tpt, i);
+      const int ulo = b.cnt[0] > 0 ? b.lo[0] : b.lo[1];
+      const int uhi = max(b.cnt[0] > 0 ? b.lo[0] + b.cnt[0] - 1 : 0, b.cnt[1] > 0 ? b.lo[1] + b.cnt[1] - 1 : 0);
+      if (b.cnt[0] + b.cnt[1] == 0) continue;
+      int u[2] = {0, 0};         // key tiles whose S has been issued
+      int vit[2] = {0, 0}, vj[2] = {0, 0};
+      for (int t = 0; t < 2 && ok; ++t)
+        if (b.cnt[t] > 0) ok = warp_wait(&q_full[t], q_n[t]++ & 1, s_abort, ZS_DEVERR_TIMEOUT_MMA);
+      // O_t += P_t V of the query tile's last key tile; then that V is released for it
+      auto pv = [&](int t) -> bool {
+        const int vs = vit[t] % SLOTS;
+        uint8_t* v = smem + L::OFF_KV + vs * L::TILE;
+        if (!warp_wait(&kv_full[vs], (vit[t] / SLOTS) & 1, s_abort, ZS_DEVERR_TIMEOUT_MMA)) return false;
+        // Values of keys that no query sees (behind the sequence, before every window) count as zero,
+        // whatever lies there: 0 * NaN would reach every row.
+        const int k0 = vj[t] * PT_KEYS;
+        if (k0 + PT_KEYS > b.len || k0 < b.floor) {
+          for (int r = 0; r < PT_KEYS; ++r) {
+            if (k0 + r < b.len && k0 + r >= b.floor) continue;
+            if (lane < 8 * ATOMS)
+              *reinterpret_cast<uint4*>(v + (lane >> 3) * ATOM + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        // the first product of a block overwrites O: the last block's rows must be out
+        if (u[t] == 1 && !warp_wait(&o_free[t], (b_n[t] & 1) ^ 1, s_abort, ZS_DEVERR_TIMEOUT_MMA)) return false;
+        const uint32_t va = smem_u32(v);
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          if (!warp_wait(hf == 0 ? &p_half[t] : &p_full[t], p_n[t] & 1, s_abort, ZS_DEVERR_TIMEOUT_MMA)) return false;
+          tc_fence_after();
+          if (lane == 0) {
+#pragma unroll
+            for (int kk = hf * 4; kk < hf * 4 + 4; ++kk)
+              tc_mma_f16_ts(tmem + 256 + t * HD, tmem + t * 128 + kk * 8, smem_desc(va + kk * 2048, ATOM, 1024, 2),
+                            IDESC_PV, (u[t] > 1 || kk > 0) ? 1u : 0u);
+          }
+          __syncwarp();
+        }
+        ++p_n[t];
+        if (lane == 0) tc_commit(&kv_empty[vs]);
+        __syncwarp();
+        return true;
+      };
+      for (int j = ulo; ok && j <= uhi; ++j) {
+        const bool in[2] = {j >= b.lo[0] && j < b.lo[0] + b.cnt[0], j >= b.lo[1] && j < b.lo[1] + b.cnt[1]};
+        if (!in[0] && !in[1]) continue;
+        const int ks = item % SLOTS, iv = item + 1;
+        if (!warp_wait(&kv_full[ks], (item / SLOTS) & 1, s_abort, ZS_DEVERR_TIMEOUT_MMA)) {
+          ok = false;
+          break;
+        }
+        item += 2;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (!in[t]) {
+            if (lane == 0) tc_commit(&kv_empty[iv % SLOTS]);   // never reads this V
+            __syncwarp();
+            continue;
+          }
+          if (u[t] > 0 && !pv(t)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          if (lane == 0) {
+            const uint32_t qa = smem_u32(smem + L::OFF_Q + t * L::TILE);
+            const uint32_t ka = smem_u32(smem + L::OFF_KV + ks * L::TILE);
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; ++kk) {
+              const uint32_t off = (kk / 4) * ATOM + (kk % 4) * 32;
+              tc_mma_f16(tmem + t * 128, smem_desc(qa + off, 16, 1024, 2), smem_desc(ka + off, 16, 1024, 2), IDESC_S,
+                         kk > 0 ? 1u : 0u);
+            }
+            tc_commit(&s_full[t]);
+            if (u[t] + 1 == b.cnt[t]) tc_commit(&q_empty[t]);   // the block's last use of this Q
+            issued_any = true;
+          }
+          __syncwarp();
+          ++u[t];
+          vit[t] = iv;
+          vj[t] = j;
+        }
+        if (!ok) break;
+        if (lane == 0) {
+          tc_commit(&kv_empty[ks]);
+          tc_commit(&kv_empty[ks]);
+        }
+        __syncwarp();
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (!ok || u[t] == 0) continue;
+        ok = pv(t);
+        if (lane == 0) tc_commit(&o_done[t]);
+        __syncwarp();
+        ++b_n[t];
+      }
+    }
+    if (__any_sync(0xffffffffu, issued_any)) {
+      if (lane == 0) {
+        tc_commit(done);
+        mbar_wait(done, 0, nullptr, ZS_DEVERR_TIMEOUT_DRAIN);
+      }
+      __syncwarp();
+    }
+  } else {
+    // ------------------------------------------------------------------ rows of no sequence
+    const int64_t end = cut_row(a, a.num_seqs), begin = cut_row(a, 0);
+    const int64_t me = (int64_t)blockIdx.x * 64 + threadIdx.x - 64, all = (int64_t)gridDim.x * 64;
+    const int64_t words = (int64_t)a.H * (HD / 8);
+    for (int64_t e = me; e < a.tokens * words; e += all) {
+      const int64_t tok = e / words;
+      if (tok >= begin && tok < end) {
+        e += (end - 1 - tok) * words / all * all;        // on to the rows behind the sequences
+        continue;
+      }
+      reinterpret_cast<uint4*>(a.o)[e] = make_uint4(0, 0, 0, 0);
+      if (a.lse != nullptr && e % (HD / 8) == 0) a.lse[e / (HD / 8)] = -INFINITY;
+    }
+  }
+  } else {
+    // ------------------------------------------------------------------ softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PT_REGS_SOFTMAX));
+    const int t = (warp - 4) >> 2;
+    const int quarter = warp & 3;
+    const int r = quarter * 32 + lane;                   // this thread's row
+    const int tr = r / G, g = r - tr * G;                // its token in the tile, its head in the group
+    const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+    const uint32_t ts = tmem + lane_base + t * 128, to = tmem + lane_base + 256 + t * HD;
+    const uint64_t scale2 = attn::pack2(__float_as_uint(a.scale_log2), __float_as_uint(a.scale_log2));
+    uint32_t s_n = 0, b_n = 0, q_n = 0;
+    bool ok = true;
+    ZS_EACH_BLOCK(i) {
+      if (!ok) break;
+      const PromptBlock b = find_block(a, sums, group, per, tpt, i);
+      const int tokens = min(b.left - t * tpt, tpt);     // of the tile
+      if (tokens <= 0) continue;
+      const bool valid = tr < tokens;
+      const int p0 = b.pos0 + t * tpt, p = p0 + tr;      // the tile's first position, the row's
+      const int h = b.hk * G + min(g, G - 1);
+      const int64_t tok = (int64_t)b.tok0 + t * tpt + tr;
+      const int n = b.cnt[t];
+      float m = -INFINITY, l = 0.f;
+      float z = 0.f;
+      if (n > 0) {
+        if (a.k_sink != nullptr) {                       // the row's sink logit, from the Q tile (swizzled 16-byte chunks)
+          if (!warp_wait(&q_full[t], q_n & 1, s_abort, ZS_DEVERR_TIMEOUT_EPILOGUE)) {
+            ok = false;
+            break;
+          }
+          const uint8_t* qrow = smem + L::OFF_Q + t * L::TILE + r * 128;
+#pragma unroll 4
+          for (int ch = 0; ch < HD / 8; ++ch) {
+            const uint4 x = *reinterpret_cast<const uint4*>(qrow + (ch >> 3) * ATOM + (((ch & 7) ^ (r & 7)) << 4));
+            float f[8], v[8];
+            unpack8<T>(x, f);
+            load_sink<4>(a, (int64_t)h * HD + ch * 8, *reinterpret_cast<float(*)[4]>(v));
+            load_sink<4>(a, (int64_t)h * HD + ch * 8 + 4, *reinterpret_cast<float(*)[4]>(v + 4));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) z = fmaf(f[e], v[e], z);
+          }
+          z *= a.scale_log2;
+        }
+        ++q_n;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_empty[t]);
+      }
+      for (int uu = 0; uu < n; ++uu) {
+        const int k0 = (b.lo[t] + uu) * PT_KEYS;
+        if (!warp_wait(&s_full[t], s_n & 1, s_abort, ZS_DEVERR_TIMEOUT_EPILOGUE)) {
+          ok = false;
+          break;
+        }
+        ++s_n;
+        tc_fence_after();
+        uint32_t sr[128];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(ts + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&sr[c * 32]));
+        tc_wait_ld();
+        const bool edge = k0 + PT_KEYS - 1 > p0 || (a.window > 0 && p0 + tokens - 1 - k0 >= a.window);
+        if (edge) {
+          const int k1 = p - k0;                                         // last and first visible column
+          const int kf = a.window > 0 ? p - (a.window - 1) - k0 : 0;
+#pragma unroll
+          for (int c = 0; c < 128; ++c)
+            if (c > k1 || c < kf) sr[c] = __float_as_uint(-INFINITY);
+        }
+        float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 128; c += 8) {
+          mx0 = attn::fmax3(mx0, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
+          mx1 = attn::fmax3(mx1, __uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3]));
+          mx2 = attn::fmax3(mx2, __uint_as_float(sr[c + 4]), __uint_as_float(sr[c + 5]));
+          mx3 = attn::fmax3(mx3, __uint_as_float(sr[c + 6]), __uint_as_float(sr[c + 7]));
+        }
+        const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * a.scale_log2;
+        const bool need = mx > m + 8.0f;
+        float f = 1.0f;
+        if (need) {
+          f = m == -INFINITY ? 0.f : attn::fast_exp2(m - mx);
+          l *= f;
+          m = mx;
+        }
+        // O_t holds every earlier product of the block (this S_t was issued after them)
+        if (uu >= 1 && __any_sync(0xffffffffu, need)) {
+#pragma unroll 1
+          for (int c = 0; c < HD / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld_32x32b_x32(to + c * 32, o);
+            tc_wait_ld();
+#pragma unroll
+            for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+            attn::tmem_st_32x32b_x32(to + c * 32, o);
+          }
+        }
+        const float mu = m == -INFINITY ? 0.f : m;        // nothing seen so far: every P is exp2(-inf)
+        const uint64_t negm = attn::pack2(__float_as_uint(-mu), __float_as_uint(-mu));
+        uint64_t acc0 = 0, acc1 = 0;
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          uint32_t pw[32];
+#pragma unroll
+          for (int x = 0; x < 32; x += 2) {
+            const int c = hf * 64 + 2 * x;
+            float e0, e1, e2, e3;
+            attn::unpack2(attn::ffma2(attn::pack2(sr[c], sr[c + 1]), scale2, negm), e0, e1);
+            attn::unpack2(attn::ffma2(attn::pack2(sr[c + 2], sr[c + 3]), scale2, negm), e2, e3);
+            e0 = attn::fast_exp2(e0);
+            e1 = attn::fast_exp2(e1);
+            e2 = attn::fast_exp2(e2);
+            e3 = attn::fast_exp2(e3);
+            acc0 = attn::fadd2(acc0, attn::pack2(__float_as_uint(e0), __float_as_uint(e1)));
+            acc1 = attn::fadd2(acc1, attn::pack2(__float_as_uint(e2), __float_as_uint(e3)));
+            const typename Pair<T>::type p01 = Pair<T>::from_f(e0, e1), p23 = Pair<T>::from_f(e2, e3);
+            pw[x] = *reinterpret_cast<const uint32_t*>(&p01);
+            pw[x + 1] = *reinterpret_cast<const uint32_t*>(&p23);
+          }
+          attn::tmem_st_32x32b_x32(ts + hf * 32, pw);
+          attn::tc_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(hf == 0 ? &p_half[t] : &p_full[t]);
+        }
+        float a0, a1, a2, a3;
+        attn::unpack2(acc0, a0, a1);
+        attn::unpack2(acc1, a2, a3);
+        l += (a0 + a1) + (a2 + a3);
+      }
+      if (!ok) break;
+      float f = 1.f;
+      if (a.k_sink != nullptr) {
+        const float mt = fmaxf(m, z);
+        f = m == -INFINITY ? 0.f : attn::fast_exp2(m - mt);
+        l = l * f + attn::fast_exp2(z - mt);
+        m = mt;
+      }
+      float inv = l > 0.f ? f / l : (l != l ? l : 0.f);
+      if (valid) {
+        inv *= gate_of<T>(a, tok, h);
+        if (a.lse != nullptr)
+          a.lse[tok * a.H + h] = l > 0.f ? (m + log2f(l)) * 0.6931471805599453f : (l != l ? l : -INFINITY);
+      }
+      T* out = reinterpret_cast<T*>(a.o) + (tok * a.H + h) * HD;
+      if (n == 0) {                                      // all before the sequence's first position
+        if (valid)
+          for (int c = 0; c < HD; c += 8) *reinterpret_cast<uint4*>(out + c) = make_uint4(0, 0, 0, 0);
+        continue;
+      }
+      if (!warp_wait(&o_done[t], b_n & 1, s_abort, ZS_DEVERR_TIMEOUT_EPILOGUE)) {
+        ok = false;
+        break;
+      }
+      ++b_n;
+      tc_fence_after();
+#pragma unroll 1
+      for (int c = 0; c < HD / 32; ++c) {
+        uint32_t o[32];
+        tmem_ld_32x32b_x32(to + c * 32, o);
+        tc_wait_ld();
+        if (valid) {
+          uint4* dst = reinterpret_cast<uint4*>(out + c * 32);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            float v[8];
+#pragma unroll
+            for (int y = 0; y < 8; ++y) v[y] = __uint_as_float(o[x * 8 + y]) * inv;
+            dst[x] = pack8<T>(v);
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&o_free[t]);
+    }
+  }
+#undef ZS_EACH_BLOCK
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
 }  // namespace paged
 }  // namespace zs
 
@@ -825,26 +1293,15 @@ static int attn_args(paged::AttnArgs& a, const void* q, int64_t ldq, const void*
   return ZS_OK;
 }
 
-static int launch_plain(const paged::AttnArgs& a, int hd, int dtype, cudaStream_t stream) {
-  const dim3 grid((unsigned)a.tokens, (unsigned)a.H);
-  if (dtype == ZS_BF16) {
-    if (hd == 128) paged::paged_attn_kernel<__nv_bfloat16, 128><<<grid, 128, 0, stream>>>(a);
-    else paged::paged_attn_kernel<__nv_bfloat16, 64><<<grid, 128, 0, stream>>>(a);
-  } else {
-    if (hd == 128) paged::paged_attn_kernel<__half, 128><<<grid, 128, 0, stream>>>(a);
-    else paged::paged_attn_kernel<__half, 64><<<grid, 128, 0, stream>>>(a);
-  }
-  ZS_CUDA_TRY(cudaGetLastError());
-  return ZS_OK;
-}
-
-static int make_page_tmap(CUtensorMap* m, const void* base, int dtype, int hd, int64_t rows, int64_t pages,
-                          int64_t page_stride, int box_rows) {
+// 3-D tensor map of 16-bit elements [n2][n1][hd] with element strides ld2 and ld1, boxes of
+// box2 x box1 rows of 64 elements, 128-byte swizzle.
+static int make_tmap3(CUtensorMap* m, const void* base, int dtype, int hd, int64_t n1, int64_t n2, int64_t ld1,
+                      int64_t ld2, int box1, int box2) {
   auto fn = encode_fn();
   if (fn == nullptr) return ZS_ERR_CUDA;
-  cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)rows, (cuuint64_t)pages};
-  cuuint64_t strides[2] = {(cuuint64_t)hd * 2, (cuuint64_t)page_stride * 2};
-  cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1};
+  cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)n1, (cuuint64_t)n2};
+  cuuint64_t strides[2] = {(cuuint64_t)ld1 * 2, (cuuint64_t)ld2 * 2};
+  cuuint32_t box[3] = {64, (cuuint32_t)box1, (cuuint32_t)box2};
   cuuint32_t es[3] = {1, 1, 1};
   const CUresult r = fn(m, dtype == ZS_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
                         const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -855,6 +1312,12 @@ static int make_page_tmap(CUtensorMap* m, const void* base, int dtype, int hd, i
     return ZS_ERR_CUDA;
   }
   return ZS_OK;
+}
+
+// Pages of one layer's keys or values: rows [Hkv * page] of a page, boxes of one page's rows.
+static int make_page_tmap(CUtensorMap* m, const void* base, int dtype, int hd, int64_t rows, int64_t pages,
+                          int64_t page_stride, int box_rows) {
+  return make_tmap3(m, base, dtype, hd, rows, pages, hd, page_stride, box_rows, 1);
 }
 
 template <typename T, int HD>
@@ -908,6 +1371,25 @@ extern "C" int zs_paged_decode_attention(const void* q, int64_t ldq, const void*
                    : launch_decode<__half, 64>(a, dtype, workspace, stream);
 }
 
+template <typename T, int HD>
+static int launch_prompt(const paged::AttnArgs& a, int dtype, cudaStream_t stream) {
+  using L = paged::PromptSmem<HD>;
+  const int G = a.H / a.Hkv, tpt = paged::PT_ROWS / G, box = a.page < paged::PT_KEYS ? a.page : paged::PT_KEYS;
+  CUtensorMap tq, tk, tv;
+  int rc = make_tmap3(&tq, a.q, dtype, HD, a.H, a.tokens, HD, a.ldq, G, tpt);
+  if (rc != ZS_OK) return rc;
+  rc = make_page_tmap(&tk, a.k_pages, dtype, HD, (int64_t)a.Hkv * a.page, a.num_pages, a.page_stride, box);
+  if (rc != ZS_OK) return rc;
+  rc = make_page_tmap(&tv, a.v_pages, dtype, HD, (int64_t)a.Hkv * a.page, a.num_pages, a.page_stride, box);
+  if (rc != ZS_OK) return rc;
+  const int64_t most = (a.tokens / (2 * tpt) + a.num_seqs) * a.Hkv;      // blocks that the packed rows can make
+  const int grid = (int)(most < num_sms() ? most : num_sms());
+  ZS_CUDA_TRY(cudaFuncSetAttribute(paged::paged_prompt_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::ALLOC));
+  paged::paged_prompt_kernel<T, HD><<<grid, paged::PT_THREADS, L::ALLOC, stream>>>(tq, tk, tv, a);
+  ZS_CUDA_TRY(cudaGetLastError());
+  return ZS_OK;
+}
+
 extern "C" int zs_paged_prompt_attention(const void* q, int64_t ldq, const void* k_pages, const void* v_pages,
                                          int64_t page_stride, int64_t num_pages, const int* block_table,
                                          int64_t bt_ld, int max_pages, const int* seq_lens, const int* cu_seqlens,
@@ -921,6 +1403,10 @@ extern "C" int zs_paged_prompt_attention(const void* q, int64_t ldq, const void*
                            cu_seqlens, num_seqs, tokens, H, Hkv, hd, page, window, scale, k_sink, sink_dtype, gate,
                            ldg, o, lse, dtype);
   if (rc != ZS_OK) return rc;
+  ZS_REQUIRE(H / Hkv <= paged::PT_ROWS, ZS_ERR_SHAPE);
   ZS_BIND(q);
-  return launch_plain(a, hd, dtype, stream);
+  if (dtype == ZS_BF16)
+    return hd == 128 ? launch_prompt<__nv_bfloat16, 128>(a, dtype, stream)
+                     : launch_prompt<__nv_bfloat16, 64>(a, dtype, stream);
+  return hd == 128 ? launch_prompt<__half, 128>(a, dtype, stream) : launch_prompt<__half, 64>(a, dtype, stream);
 }

@@ -178,8 +178,11 @@ def _attention(q, k_pages, v_pages, block_table, seq_lens, cu_seqlens, window, k
     if len(shape) != 3 or q.dtype != dtype or shape[2] != hd or shape[1] < 1 or shape[1] % Hkv:
         _fail(f"q must be {dtype} [T, H, {hd}] with H % Hkv == 0 (got {q.dtype} {tuple(shape)}, Hkv={Hkv})")
     T, H, _ = shape
-    if decode and T != n:
-        _fail(f"q has one row per sequence (got {T} rows, {n} sequences)")
+    if decode:
+        if T != n:
+            _fail(f"q has one row per sequence (got {T} rows, {n} sequences)")
+    elif H // Hkv > 128:
+        _fail(f"at most 128 query heads share a key head (got H={H}, Hkv={Hkv})")
     w = 0
     if window is not None:
         w = int(window)

@@ -691,6 +691,7 @@ int zs_sparse_rmsprop_step(float* param, int64_t num_rows, int64_t d, int64_t ld
  *   key: o is zero (lse of padding outside every sequence: -inf).  A NaN or
  *   infinity in a value of the sequence may reach every row of the same
  *   sequence; what lies in the pages outside the sequence reaches none.
+ *   H / Hkv <= 128.
  * zs_paged_decode_attention: the same for one token per sequence (row s), with
  *   the keys of a sequence split over blocks and joined in a fixed order;
  *   seq_lens[s] == 0 marks an empty slot (o zero).  The workspace holds partial
