@@ -720,6 +720,43 @@ constexpr int PT_THREADS = 384;
 constexpr int PT_REGS_AUX = 104, PT_REGS_SOFTMAX = 200;
 constexpr int PT_SUMS = 256;              // sequence groups whose block counts lie in shared memory
 
+// One lane of the converged warp; the compiler keeps what the branch computes in uniform registers,
+// where the tensor instructions want their descriptors.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r)::"memory");
+  return r != 0;
+}
+// Products with the descriptors' low words as arguments (address and leading offset; the high word,
+// stride 1024 bytes and 128-byte swizzle, is the same for all): one addition per operand and step.
+constexpr uint32_t DESC_HI = (1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(const void* p, uint32_t lead) {
+  return (smem_u32(p) >> 4 & 0x3FFF) | (lead >> 4) << 16;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 da, {%1, %3};\n\t"
+      "mov.b64 db, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "n"(DESC_HI), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 db, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b_lo), "n"(DESC_HI), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
 template <int HD>
 struct PromptSmem {
   static constexpr int TILE = 128 * HD * 2;
@@ -743,6 +780,7 @@ struct PromptBlock {
   int len;                 // tokens in the cache (cut)
   int floor;               // no query of the sequence sees a key before this one
   int lo[2], cnt[2];       // key tiles of the two query tiles
+  int first, last;         // of both: one range (a window reaches back at least to the token itself)
 };
 
 // Packed row i of cu_seqlens, inside the rows there are.
@@ -786,6 +824,8 @@ __device__ __forceinline__ PromptBlock find_block(const AttnArgs& a, const int* 
     b.lo[t] = (a.window > 0 ? max(p0 - (a.window - 1), 0) : 0) / PT_KEYS;
     b.cnt[t] = rows > 0 && p1 >= 0 ? p1 / PT_KEYS - b.lo[t] + 1 : 0;
   }
+  b.first = b.cnt[0] > 0 ? b.lo[0] : b.lo[1];
+  b.last = b.cnt[1] > 0 ? b.lo[1] + b.cnt[1] - 1 : b.lo[0] + b.cnt[0] - 1;
   return b;
 }
 
@@ -833,7 +873,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     }
     for (int s = 0; s < SLOTS; ++s) {
       mbar_init(&kv_full[s], 1);
-      mbar_init(&kv_empty[s], 2);                        // one release per query tile
+      mbar_init(&kv_empty[s], 1);
     }
     mbar_init(done, 1);
     *s_abort = 0;
@@ -882,10 +922,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     ZS_EACH_BLOCK(i) {
       if (!ok) break;
       const PromptBlock b = find_block(a, sums, group, per, tpt, i);
-      for (int t = 0; t < 2 && ok; ++t) {
-        if (b.cnt[t] == 0) continue;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (!ok || b.cnt[t] == 0) continue;
         ok = warp_wait(&q_empty[t], (q_n[t] & 1) ^ 1, s_abort, ZS_DEVERR_TIMEOUT_PRODUCER);
-        if (!ok) break;
+        if (!ok) continue;
         if (lane == 0) {
           mbar_arrive_expect_tx(&q_full[t], G * tpt * HD * 2);
 #pragma unroll
@@ -895,11 +936,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
         }
         ++q_n[t];
       }
-      const int ulo = b.cnt[0] > 0 ? b.lo[0] : b.lo[1];
-      const int uhi = max(b.cnt[0] > 0 ? b.lo[0] + b.cnt[0] - 1 : 0, b.cnt[1] > 0 ? b.lo[1] + b.cnt[1] - 1 : 0);
       if (b.cnt[0] + b.cnt[1] == 0) continue;
-      for (int j = ulo; ok && j <= uhi; ++j) {
-        if (!(j >= b.lo[0] && j < b.lo[0] + b.cnt[0]) && !(j >= b.lo[1] && j < b.lo[1] + b.cnt[1])) continue;
+      for (int j = b.first; ok && j <= b.last; ++j) {
         const int key = j * PT_KEYS + pg * rows;
         int page = (int)a.num_pages;                     // past the pool: TMA fills zeros
         if (lane < boxes && key < b.len && key + rows > b.floor) {
@@ -927,6 +965,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
       }
     }
     // copies in flight land before the CTA leaves
+#pragma unroll
     for (int t = 0; t < 2; ++t)
       if (q_n[t] > 0) mbar_wait(&q_full[t], (q_n[t] - 1) & 1, nullptr, ZS_DEVERR_TIMEOUT_DRAIN);
     for (int s = 0; s < SLOTS; ++s)
@@ -934,114 +973,102 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
   } else if (warp == 1) {
     // ------------------------------------------------------------------ products
     bool ok = true, issued_any = false;
-    int item = 0;
+    int item = 0;                // of the ring: the block's first K
     uint32_t q_n[2] = {0, 0};    // Q tiles waited for
     uint32_t p_n[2] = {0, 0};    // P tiles waited for
     uint32_t b_n[2] = {0, 0};    // blocks begun, per query tile
+    const uint32_t q_lo = desc_lo(smem + L::OFF_Q, 16), k_lo = desc_lo(smem + L::OFF_KV, 16),
+                   v_lo = desc_lo(smem + L::OFF_KV, ATOM);
+    auto ready = [&](int it) -> bool {
+      return warp_wait(&kv_full[it % SLOTS], (it / SLOTS) & 1, s_abort, ZS_DEVERR_TIMEOUT_MMA);
+    };
     ZS_EACH_BLOCK(i) {
       if (!ok) break;
       const PromptBlock b = find_block(a, sums, group, per, tpt, i);
-      const int ulo = b.cnt[0] > 0 ? b.lo[0] : b.lo[1];
-      const int uhi = max(b.cnt[0] > 0 ? b.lo[0] + b.cnt[0] - 1 : 0, b.cnt[1] > 0 ? b.lo[1] + b.cnt[1] - 1 : 0);
       if (b.cnt[0] + b.cnt[1] == 0) continue;
-      int u[2] = {0, 0};         // key tiles whose S has been issued
-      int vit[2] = {0, 0}, vj[2] = {0, 0};
-      for (int t = 0; t < 2 && ok; ++t)
-        if (b.cnt[t] > 0) ok = warp_wait(&q_full[t], q_n[t]++ & 1, s_abort, ZS_DEVERR_TIMEOUT_MMA);
-      // O_t += P_t V of the query tile's last key tile; then that V is released for it
-      auto pv = [&](int t) -> bool {
-        const int vs = vit[t] % SLOTS;
-        uint8_t* v = smem + L::OFF_KV + vs * L::TILE;
-        if (!warp_wait(&kv_full[vs], (vit[t] / SLOTS) & 1, s_abort, ZS_DEVERR_TIMEOUT_MMA)) return false;
-        // Values of keys that no query sees (behind the sequence, before every window) count as zero,
-        // whatever lies there: 0 * NaN would reach every row.
-        const int k0 = vj[t] * PT_KEYS;
-        if (k0 + PT_KEYS > b.len || k0 < b.floor) {
-          for (int r = 0; r < PT_KEYS; ++r) {
-            if (k0 + r < b.len && k0 + r >= b.floor) continue;
-            if (lane < 8 * ATOMS)
-              *reinterpret_cast<uint4*>(v + (lane >> 3) * ATOM + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-        }
-        // the first product of a block overwrites O: the last block's rows must be out
-        if (u[t] == 1 && !warp_wait(&o_free[t], (b_n[t] & 1) ^ 1, s_abort, ZS_DEVERR_TIMEOUT_MMA)) return false;
-        const uint32_t va = smem_u32(v);
+      const int ulo = b.first, uhi = b.last;
+      const int end[2] = {b.lo[0] + b.cnt[0], b.lo[1] + b.cnt[1]};
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          if (!warp_wait(hf == 0 ? &p_half[t] : &p_full[t], p_n[t] & 1, s_abort, ZS_DEVERR_TIMEOUT_MMA)) return false;
-          tc_fence_after();
-          if (lane == 0) {
-#pragma unroll
-            for (int kk = hf * 4; kk < hf * 4 + 4; ++kk)
-              tc_mma_f16_ts(tmem + 256 + t * HD, tmem + t * 128 + kk * 8, smem_desc(va + kk * 2048, ATOM, 1024, 2),
-                            IDESC_PV, (u[t] > 1 || kk > 0) ? 1u : 0u);
-          }
-          __syncwarp();
-        }
-        ++p_n[t];
-        if (lane == 0) tc_commit(&kv_empty[vs]);
-        __syncwarp();
-        return true;
-      };
-      for (int j = ulo; ok && j <= uhi; ++j) {
-        const bool in[2] = {j >= b.lo[0] && j < b.lo[0] + b.cnt[0], j >= b.lo[1] && j < b.lo[1] + b.cnt[1]};
-        if (!in[0] && !in[1]) continue;
-        const int ks = item % SLOTS, iv = item + 1;
-        if (!warp_wait(&kv_full[ks], (item / SLOTS) & 1, s_abort, ZS_DEVERR_TIMEOUT_MMA)) {
-          ok = false;
-          break;
-        }
-        item += 2;
+      for (int t = 0; t < 2; ++t)
+        if (ok && b.cnt[t] > 0) ok = warp_wait(&q_full[t], q_n[t]++ & 1, s_abort, ZS_DEVERR_TIMEOUT_MMA);
+      ok = ok && ready(item);
+      // Step j: per query tile O_t += P_t V_{j-1}, then S_t = Q_t K_j; what step j + 1 reads is waited for
+      // between the two query tiles, where the tensor pipe has work queued.
+      int ks = item % SLOTS, vs = 0;
+      for (int j = ulo; ok && j <= uhi + 1; ++j) {
+        int ks_next = 0, vs_next = 0;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          if (!in[t]) {
-            if (lane == 0) tc_commit(&kv_empty[iv % SLOTS]);   // never reads this V
-            __syncwarp();
-            continue;
-          }
-          if (u[t] > 0 && !pv(t)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          if (lane == 0) {
-            const uint32_t qa = smem_u32(smem + L::OFF_Q + t * L::TILE);
-            const uint32_t ka = smem_u32(smem + L::OFF_KV + ks * L::TILE);
+          if (ok && j - 1 >= b.lo[t] && j - 1 < end[t]) {
+            // the block's first product overwrites O: the last block's rows must be out
+            const bool fresh = j - 1 == b.lo[t];
+            if (fresh) ok = warp_wait(&o_free[t], (b_n[t]++ & 1) ^ 1, s_abort, ZS_DEVERR_TIMEOUT_MMA);
+            const uint32_t va = v_lo + vs * (L::TILE >> 4);
 #pragma unroll
-            for (int kk = 0; kk < HD / 16; ++kk) {
-              const uint32_t off = (kk / 4) * ATOM + (kk % 4) * 32;
-              tc_mma_f16(tmem + t * 128, smem_desc(qa + off, 16, 1024, 2), smem_desc(ka + off, 16, 1024, 2), IDESC_S,
-                         kk > 0 ? 1u : 0u);
+            for (int hf = 0; hf < 2; ++hf) {
+              ok = ok && warp_wait(hf == 0 ? &p_half[t] : &p_full[t], p_n[t] & 1, s_abort, ZS_DEVERR_TIMEOUT_MMA);
+              tc_fence_after();
+              if (ok && elect_one()) {
+#pragma unroll
+                for (int kk = hf * 4; kk < hf * 4 + 4; ++kk)
+                  mma_ts(tmem + 256 + t * HD, tmem + t * 128 + kk * 8, va + kk * (2048 >> 4), IDESC_PV,
+                         kk > 0 ? 1u : (fresh ? 0u : 1u));
+                if (hf == 1 && j == end[t]) tc_commit(&o_done[t]);
+              }
+              __syncwarp();
             }
-            tc_commit(&s_full[t]);
-            if (u[t] + 1 == b.cnt[t]) tc_commit(&q_empty[t]);   // the block's last use of this Q
-            issued_any = true;
+            ++p_n[t];
           }
-          __syncwarp();
-          ++u[t];
-          vit[t] = iv;
-          vj[t] = j;
-        }
-        if (!ok) break;
-        if (lane == 0) {
-          tc_commit(&kv_empty[ks]);
-          tc_commit(&kv_empty[ks]);
-        }
-        __syncwarp();
-      }
+          if (ok && j >= b.lo[t] && j < end[t]) {
+            tc_fence_after();
+            if (elect_one()) {
+              const uint32_t qa = q_lo + t * (L::TILE >> 4), ka = k_lo + ks * (L::TILE >> 4);
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        if (!ok || u[t] == 0) continue;
-        ok = pv(t);
-        if (lane == 0) tc_commit(&o_done[t]);
-        __syncwarp();
-        ++b_n[t];
+              for (int kk = 0; kk < HD / 16; ++kk) {
+                const uint32_t off = (kk / 4) * (ATOM >> 4) + (kk % 4) * (32 >> 4);
+                mma_ss(tmem + t * 128, qa + off, ka + off, IDESC_S, kk > 0 ? 1u : 0u);
+              }
+              tc_commit(&s_full[t]);
+              if (j + 1 == end[t]) tc_commit(&q_empty[t]);     // the block's last use of this Q
+            }
+            issued_any = true;
+            __syncwarp();
+          }
+          if (t == 1 && elect_one()) {                         // both query tiles have read these
+            if (j <= uhi) tc_commit(&kv_empty[ks]);
+            if (j > ulo) tc_commit(&kv_empty[vs]);
+          }
+          if (t == 0 && ok) {
+            if (j <= uhi) {
+              vs_next = (item + 1) % SLOTS;
+              ok = ready(item + 1);
+              // Values of keys that no query sees (behind the sequence, before every window) count as zero,
+              // whatever lies there: 0 * NaN would reach every row.
+              const int k0 = j * PT_KEYS;
+              if (k0 + PT_KEYS > b.len || k0 < b.floor) {
+                uint8_t* v = smem + L::OFF_KV + vs_next * L::TILE;
+                for (int r = 0; r < PT_KEYS; ++r) {
+                  if (k0 + r < b.len && k0 + r >= b.floor) continue;
+                  if (lane < 8 * ATOMS)
+                    *reinterpret_cast<uint4*>(v + (lane >> 3) * ATOM + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+              }
+            }
+            if (j < uhi) {
+              ks_next = (item + 2) % SLOTS;
+              ok = ok && ready(item + 2);
+            }
+          }
+        }
+        ks = ks_next;
+        vs = vs_next;
+        if (j <= uhi) item += 2;
       }
     }
-    if (__any_sync(0xffffffffu, issued_any)) {
-      if (lane == 0) {
+    if (issued_any) {                                    // what was issued ends before the warp leaves
+      if (elect_one()) {
         tc_commit(done);
         mbar_wait(done, 0, nullptr, ZS_DEVERR_TIMEOUT_DRAIN);
       }
@@ -1083,7 +1110,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
       const int p0 = b.pos0 + t * tpt, p = p0 + tr;      // the tile's first position, the row's
       const int h = b.hk * G + min(g, G - 1);
       const int64_t tok = (int64_t)b.tok0 + t * tpt + tr;
-      const int n = b.cnt[t];
+      const int n = t == 0 ? b.cnt[0] : b.cnt[1], lo = t == 0 ? b.lo[0] : b.lo[1];
       float m = -INFINITY, l = 0.f;
       float z = 0.f;
       if (n > 0) {
@@ -1110,7 +1137,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
         if (lane == 0) mbar_arrive(&q_empty[t]);
       }
       for (int uu = 0; uu < n; ++uu) {
-        const int k0 = (b.lo[t] + uu) * PT_KEYS;
+        const int k0 = (lo + uu) * PT_KEYS;
         if (!warp_wait(&s_full[t], s_n & 1, s_abort, ZS_DEVERR_TIMEOUT_EPILOGUE)) {
           ok = false;
           break;
