@@ -12,6 +12,9 @@ QK-norm + RoPE of q and k and the tcgen05 flash attention reading v and the gate
 logits in place from the projection output, with the sigmoid gate applied in its
 epilogue (backward: the attention kernels and the norm/RoPE transpose write the
 projection output's gradient directly); and the output projection.
+
+forward_paged answers from a paged key-value cache (zs_b200.paged): new tokens' keys
+and values go to their pages, and attention reads the pages.
 """
 from __future__ import annotations
 
@@ -24,6 +27,7 @@ import torch.nn.functional as F
 from zs_b200.attn import attention as attention_core
 from zs_b200.attn import gated_attention_core
 from zs_b200.dense import dense_linear
+from zs_b200.paged import paged_append, paged_decode_attention, paged_prompt_attention
 
 from .liger_rope import LigerRopeFunction, PartialRopeFunction  # noqa: F401
 from .zRMSNorm import ZeroCenteredRMSNorm
@@ -165,3 +169,26 @@ class GatedAttention(nn.Module):
         attn = attn * gate.unsqueeze(-1)
         return dense_linear(attn.reshape(bsz, seq_len, self.num_heads * self.head_dim), [self.o_proj.weight],
                             tag="proj_o")
+
+    def forward_paged(self, hidden_states, k_pages, v_pages, block_table, seq_lens, cu_seqlens=None):
+        """The layer on packed new tokens [1, T, d] whose keys and values are stored in a paged cache
+        and read from it (no gradient).  seq_lens counts the new tokens; cu_seqlens [num_seqs + 1]
+        are the packed rows of each sequence, None one row per sequence (a decode step)."""
+        H, Hkv, hd = self.num_heads, self.num_key_value_heads, self.head_dim
+        qd, kd = H * hd, Hkv * hd
+        ws = [self.q_proj.weight, self.k_proj.weight, self.v_proj.weight, self.head_gate_proj.weight]
+        qkvg = dense_linear(hidden_states, ws, tag="proj_qkvg", pad=-(qd + 2 * kd + H) % 16)[0]
+        cos = sin = None
+        if self.do_rope and self.pos_rope_pairs > 0:
+            cos, sin = self.pos_cos_cache[:, :self.pos_rope_pairs], self.pos_sin_cache[:, :self.pos_rope_pairs]
+        norm = {}
+        if self.use_qk_norm:
+            norm = dict(q_weight=self.q_norm.weight, k_weight=self.k_norm.weight, eps=self.q_norm.eps)
+        q = paged_append(qkvg, k_pages, v_pages, block_table, seq_lens, n_heads=H, cu_seqlens=cu_seqlens, cos=cos,
+                         sin=sin, **norm)
+        more = dict(window=self.window_size, k_sink=self.k_sink, gate=qkvg[:, qd + 2 * kd:qd + 2 * kd + H])
+        if cu_seqlens is None:
+            attn = paged_decode_attention(q, k_pages, v_pages, block_table, seq_lens, **more)
+        else:
+            attn = paged_prompt_attention(q, k_pages, v_pages, block_table, seq_lens, cu_seqlens, **more)
+        return dense_linear(attn.view(1, -1, qd), [self.o_proj.weight], tag="proj_o")

@@ -48,3 +48,14 @@ class TransformerBlock(nn.Module):
             attn = attn.to(torch.bfloat16)
         h, y2 = AddZRMSNormFunction.apply(x, attn, n2.weight, n2.eps)
         return self.mlp(y2, unpad_indices=unpad_indices, out_dtype=torch.float32, residual=h)
+
+    def forward_paged(self, x, k_pages, v_pages, block_table, seq_lens, cu_seqlens=None):
+        """The block on packed new tokens [1, T, d] from a paged key-value cache (no gradient)."""
+        n1, n2 = self.input_layernorm, self.post_attention_layernorm
+        pages = (k_pages, v_pages, block_table, seq_lens, cu_seqlens)
+        if not self._fused_path(x):
+            h = x + self.self_attn.forward_paged(n1(x), *pages).to(x.dtype)
+            return h + self.mlp(n2(h))[0]
+        attn = self.self_attn.forward_paged(AddZRMSNormFunction.apply(x, None, n1.weight, n1.eps), *pages)
+        h, y2 = AddZRMSNormFunction.apply(x, attn, n2.weight, n2.eps)
+        return self.mlp(y2, out_dtype=torch.float32, residual=h)[0]

@@ -1,0 +1,98 @@
+"""Continuing prompts with a trained MoELM from a paged key-value cache.
+
+The reference's inference.py:25-73 runs the whole sequence again for every new
+token.  Here the prompts run once, packed, and every further step runs one token
+per sequence: the step's kernels are recorded into one CUDA graph and replayed,
+since the launches would cost more than the work.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib as Z
+from .dense import one_group_routing
+
+
+class DecodeStep:
+    """One decode step of all slots of a cache as a CUDA graph: the slots grow by `active` (0 or 1)
+    tokens, `tokens` go in, `logits` come out.  An inactive slot's row is computed and ignored; its
+    newest token's keys are overwritten, so it must not be continued later."""
+
+    def __init__(self, model, cache):
+        dev = cache.kv.device
+        n = cache.seq_lens.numel()
+        self.model, self.cache = model, cache
+        self.slots = torch.arange(n, dtype=torch.int32, device=dev)
+        self.active = torch.zeros(n, dtype=torch.int32, device=dev)
+        self.tokens = torch.zeros(n, dtype=torch.long, device=dev)
+        self.logits = None
+        self.graph = None
+
+    def _run(self):
+        c = self.cache
+        c.extend(self.slots, self.active)
+        return self.model.forward_paged(self.tokens, c, c.block_table, c.seq_lens)
+
+    def __call__(self):
+        if self.graph is None:
+            # the first step warms up every lazily made buffer outside the recording (it is a real
+            # step), then the next ones are recorded
+            self.logits = self._run()
+            # tensors that other code may drop while the graph still reads them
+            self._held = one_group_routing(self.tokens.numel(), self.tokens.device)
+            torch.cuda.current_stream(self.tokens.device).synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                self._static = self._run()
+            self.graph = graph
+            return self.logits
+        self.graph.replay()
+        self.logits = self._static
+        return self.logits
+
+
+def sample(logits, temperature=0.0, generator=None):
+    """Token ids [n]: the largest logit (the lowest id of equals), or with a temperature a draw from
+    softmax(logits / temperature)."""
+    if temperature <= 0.0:
+        return logits.argmax(-1)
+    p = torch.softmax(logits.float() / temperature, -1)
+    return torch.multinomial(p, 1, generator=generator).squeeze(-1)
+
+
+@torch.no_grad()
+def generate(model, prompts, max_new_tokens, *, temperature=0.0, eos_token_id=None, page_size=64, generator=None):
+    """Continuations (a list of lists of ids) of prompts (a list of non-empty id sequences).  Greedy
+    by default; a sequence ends after eos_token_id (which is part of it) or max_new_tokens ids."""
+    prompts = [torch.as_tensor(p, dtype=torch.long) for p in prompts]
+    if not prompts or min(p.numel() for p in prompts) < 1:
+        raise Z.ZsError("generate needs prompts of at least one token")
+    if max_new_tokens < 1:
+        return [[] for _ in prompts]
+    dev = model.embedding.weight.device
+    lens = [p.numel() for p in prompts]
+    longest = max(lens) + max_new_tokens
+    if longest > model.config.max_position_embeddings:
+        raise Z.ZsError(f"{longest} positions exceed the model's {model.config.max_position_embeddings}")
+    cache = model.new_cache(len(prompts), longest, page_size=page_size)
+    step = DecodeStep(model, cache)
+    n_new = torch.tensor(lens, dtype=torch.int32, device=dev)
+    cu = torch.zeros(len(prompts) + 1, dtype=torch.int32, device=dev)
+    cu[1:] = n_new.cumsum(0)
+    cache.extend(step.slots, n_new)
+    logits = model.forward_paged(torch.cat(prompts).to(dev), cache, cache.block_table, cache.seq_lens, cu)
+    out = torch.full((len(prompts), max_new_tokens), -1, dtype=torch.long, device=dev)
+    step.active.fill_(1)
+    for i in range(max_new_tokens):
+        tok = sample(logits, temperature, generator)
+        out[:, i] = torch.where(step.active.bool(), tok, -1)
+        if eos_token_id is not None:
+            step.active.mul_((tok != eos_token_id).int())
+            # ask the device now and then only: the answer costs a wait
+            if i % 16 == 15 and not bool(step.active.any()):
+                break
+        if i + 1 < max_new_tokens:
+            step.tokens.copy_(tok)
+            logits = step()
+    cache.check()
+    return [[t for t in row if t >= 0] for row in out.tolist()]

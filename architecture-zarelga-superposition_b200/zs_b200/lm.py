@@ -17,7 +17,10 @@ reference's).  MoELM is the same network for machines without the reference
   produce (one value row per lookup, zs_embedding_bag_backward), which the
   sparse-row optimizer consumes without coalescing;
 * under bf16 autocast the final zero-centred RMSNorm writes bf16 directly (the
-  classifier GEMM's operand type), in the fused norm kernel.
+  classifier GEMM's operand type), in the fused norm kernel;
+* forward_paged answers from a paged key-value cache, and generate continues
+  prompts with it (zs_b200/generate.py), where the reference's inference.py:25-73
+  runs the whole sequence again for every token.
 
 Initialisation follows the reference's recipe: N(0, initializer_range) for
 every matrix, embedding rows projected to unit L2 norm, an untied head unless
@@ -130,3 +133,38 @@ class MoELM(nn.Module):
 
     def get_classifier_weights(self):
         return self.output_layer.weight
+
+    @torch.no_grad()
+    def forward_paged(self, ids, cache, block_table, seq_lens, cu_seqlens=None):
+        """Logits [num_seqs, vocab] after each sequence's last new token.  ids [T]: the packed new
+        tokens; cache: a PagedKVCache whose slots already count them (PagedKVCache.extend);
+        block_table, seq_lens: the rows of the cache's tables that belong to the sequences;
+        cu_seqlens [num_seqs + 1]: their rows in ids (None: one new token each).  Runs under bf16
+        autocast whatever the caller's context."""
+        from .dense import dense_linear
+
+        with torch.autocast("cuda", dtype=torch.bfloat16, cache_enabled=False):
+            h = self.embed(ids.view(1, -1))
+            for i, block in enumerate(self.layers):
+                h = block.forward_paged(h, *cache.layer(i), block_table, seq_lens, cu_seqlens)
+            h = self.final_norm(h)[0]
+            if cu_seqlens is not None:
+                h = h.index_select(0, (cu_seqlens[1:] - 1).clamp_min(0).long())
+            return dense_linear(h, [self.output_layer.weight], tag="logits")
+
+    def new_cache(self, max_seqs, max_tokens, *, num_pages=None, page_size=64):
+        """A PagedKVCache for this model: max_seqs slots of up to max_tokens tokens, in num_pages
+        pages (by default enough for all slots to be full)."""
+        from .paged import PagedKVCache
+
+        att = self.layers[0].self_attn
+        per_seq = -(-max_tokens // page_size)
+        return PagedKVCache(len(self.layers), att.num_key_value_heads, att.head_dim,
+                            num_pages=num_pages or max_seqs * per_seq, page_size=page_size, max_seqs=max_seqs,
+                            max_pages_per_seq=per_seq, device=self.embedding.weight.device)
+
+    def generate(self, prompts, max_new_tokens, **options):
+        """Continuations of token-id prompts; see zs_b200.generate.generate."""
+        from .generate import generate
+
+        return generate(self, prompts, max_new_tokens, **options)

@@ -1,0 +1,128 @@
+"""A model that answers: the paged path against the model's own whole-sequence forward, and
+generation through the captured decode step."""
+import pytest
+import torch
+
+from _util import rel_err
+
+pytestmark = pytest.mark.gpu
+
+
+def _model(layers=3, heads=4, kv_heads=2, windows=(None, 40, None), sink=True, qk_norm=True, rope=32):
+    from modeling.model_config import ModelConfig
+    from zs_b200.lm import MoELM
+
+    # every routed expert is chosen for every token: a rounding that swaps two experts' ranks changes nothing
+    cfg = ModelConfig(vocab_size=1024, embed_size=256, hidden_size=256, transformer_depth=layers,
+                      intermediate_size=256, n_experts=3, n_shared_experts=1, n_experts_per_token=2,
+                      n_attention_heads=heads, n_key_value_heads=kv_heads, attention_window_pattern=windows[:layers],
+                      max_position_embeddings=512, sequence_length=512, pos_rope_dims=rope, attention_sink=sink,
+                      use_qk_norm=qk_norm)
+    torch.manual_seed(0)
+    return cfg, MoELM(cfg).cuda()
+
+
+def _logits(m, ids):
+    with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16):
+        return m(ids.view(1, -1))[0][0].float()
+
+
+# The two paths run the same products in bf16 and differ where attention rounds its weights and outputs:
+# a relative 2^-8 twice per layer in one of the three summands of the residual stream, and once more in the
+# products behind it: under 2e-2 after three layers, the bound of the whole-step parity contract.
+TOL = 2e-2
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(heads=2, kv_heads=1, sink=False), dict(qk_norm=False, rope=0),
+                                dict(heads=4, kv_heads=4, windows=(7, None, 100))], ids=str)
+def test_prompt_then_steps_match_the_whole_sequence(kw):
+    from zs_b200 import _lib as Z
+
+    cfg, m = _model(**kw)
+    Z.clear_device_error()
+    g = torch.Generator(device="cuda").manual_seed(1)
+    seqs = [torch.randint(0, cfg.vocab_size, (n,), device="cuda", generator=g) for n in (150, 33, 1, 64)]
+    steps, part = 5, 20
+    more = torch.randint(0, cfg.vocab_size, (len(seqs), steps), device="cuda", generator=g)
+    c = m.new_cache(len(seqs), 256, page_size=16)
+    slots = torch.arange(len(seqs), dtype=torch.int32, device="cuda")
+
+    def run(parts):
+        n = torch.tensor([p.numel() for p in parts], dtype=torch.int32, device="cuda")
+        cu = torch.cat([n.new_zeros(1), n.cumsum(0).int()])
+        c.extend(slots, n)
+        return m.forward_paged(torch.cat(parts), c, c.block_table, c.seq_lens, cu)
+
+    # the prompts in two parts: the second reads the first from the cache
+    run([s[:part] for s in seqs])
+    got = run([s[part:] for s in seqs])
+    for i, s in enumerate(seqs):
+        if s.numel() > part:
+            assert rel_err(got[i], _logits(m, s)[-1]) < TOL
+    one = torch.ones(len(seqs), dtype=torch.int32, device="cuda")
+    for k in range(steps):
+        c.extend(slots, one)
+        got = m.forward_paged(more[:, k].contiguous(), c, c.block_table, c.seq_lens)
+        for i, s in enumerate(seqs):
+            assert rel_err(got[i], _logits(m, torch.cat([s, more[i, :k + 1]]))[-1]) < TOL
+    c.check()
+
+
+def test_fork_continues_like_its_source():
+    cfg, m = _model()
+    ids = torch.randint(0, cfg.vocab_size, (70,), device="cuda")
+    c = m.new_cache(3, 256, page_size=16)
+    n = torch.tensor([70], dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0, 70], dtype=torch.int32, device="cuda")
+    c.extend([1], n)
+    m.forward_paged(ids, c, c.block_table[1:2], c.seq_lens[1:2], cu)
+    c.fork([1, 1], [0, 2])
+    slots = torch.arange(3, dtype=torch.int32, device="cuda")
+    one = torch.ones(3, dtype=torch.int32, device="cuda")
+    for k in range(20):                      # past the end of the shared page
+        tok = torch.tensor([5, 7 + k, 5], device="cuda")
+        c.extend(slots, one)
+        out = m.forward_paged(tok, c, c.block_table, c.seq_lens)
+        assert torch.equal(out[0], out[2]) and not torch.equal(out[0], out[1])
+        if k == 9:
+            before = out
+            c.free([1])
+            c.extend([1], n)                 # the pages that slot 1 let go are used by another sequence
+            m.forward_paged(ids.flip(0).contiguous(), c, c.block_table[1:2], c.seq_lens[1:2], cu)
+            c.compact()
+    full = _logits(m, torch.cat([ids, torch.full((20,), 5, device="cuda")]))[-1]
+    assert rel_err(out[0], full) < TOL and before is not None
+    c.check()
+
+
+def test_generate_is_greedy_and_stops():
+    cfg, m = _model()
+    g = torch.Generator().manual_seed(3)
+    prompts = [torch.randint(0, cfg.vocab_size, (n,), generator=g).tolist() for n in (5, 40, 17)]
+    out = m.generate(prompts, 24)
+    assert [len(o) for o in out] == [24] * 3
+    for p, o in zip(prompts, out):
+        full = _logits(m, torch.tensor(p + o, device="cuda"))
+        for i, t in enumerate(o):
+            row = full[len(p) + i - 1]
+            # the chosen id is the largest logit, up to the paths' difference
+            assert row.max() - row[t] <= 2 * TOL * row.norm()
+    assert m.generate(prompts, 24) == out           # the captured step repeats itself
+    eos = out[0][6]
+    cut = m.generate(prompts, 24, eos_token_id=eos)
+    for o, c in zip(out, cut):
+        assert c == (o[:o.index(eos) + 1] if eos in o else o)
+    hot = m.generate(prompts[:1], 8, temperature=1.0, generator=torch.Generator(device="cuda").manual_seed(0))
+    assert len(hot[0]) == 8 and all(0 <= t < cfg.vocab_size for t in hot[0])
+
+
+def test_generate_refuses():
+    from zs_b200 import ZsError
+
+    cfg, m = _model(layers=1)
+    for bad in ([], [[]], [[1, 2], []]):
+        with pytest.raises(ZsError):
+            m.generate(bad, 4)
+    with pytest.raises(ZsError, match="positions"):
+        m.generate([[1] * 500], 100)
+    assert m.generate([[1, 2]], 0) == [[]]
