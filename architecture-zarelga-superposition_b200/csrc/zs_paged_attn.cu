@@ -700,9 +700,12 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const AttnA
 // Packed new tokens on the 5th-generation tensor cores.  The query heads of one key head share
 // its keys, so a row is a (token, head of the group) pair: a tile of 128 rows is 128 / G tokens
 // (short chunks after long prefixes fill it too), and a block is two such tiles of one
-// sequence and key head.  Blocks are numbered over all sequences from cu_seqlens on the device and
-// dealt to one persistent CTA per SM, last blocks (which see most keys) first; the loads of the
-// next block run while the rows of the last one go out.
+// sequence and key head.  As in the decode kernel the work is a list of steps, one per key tile of a
+// block (and PT_OVER for its start and end), cut on the device into equal runs, one per persistent
+// CTA: prompts of any lengths load every SM alike, and few rows after a long prefix are split over
+// its length.  Blocks that a cut goes through leave parts in the workspace, which
+// paged_prompt_join_kernel adds in the order of the CTAs.  The loads of the next block run while
+// the rows of the last one go out.
 //
 //   warp 0      TMA: both Q tiles, then K and V of 128 keys, page by page, into a ring of slots
 //   warp 1      MMA: per key tile and query tile t, O_t += P_t V (P from tensor memory, the first
@@ -718,7 +721,10 @@ constexpr int PT_THREADS = 384;
 // Registers: launched with 168 a thread (384 * 168 = 64512); the first four warps give back what
 // the softmax warps, which hold a whole row of S, take: 128 * (104 + 2 * 200) = 64512.
 constexpr int PT_REGS_AUX = 104, PT_REGS_SOFTMAX = 200;
-constexpr int PT_SUMS = 256;              // sequence groups whose block counts lie in shared memory
+constexpr int PT_PLAN = 256;              // threads that count the work
+constexpr int PT_OVER = 2;                // steps of a block's start and end
+constexpr int PT_LEAST = 6;               // steps of a run, where that leaves no block without a CTA
+constexpr int PT_MAX_CTAS = 160;
 
 // One lane of the converged warp; the compiler keeps what the branch computes in uniform registers,
 // where the tensor instructions want their descriptors.
@@ -763,8 +769,10 @@ struct PromptSmem {
   static constexpr int SLOTS = HD == 128 ? 5 : 8;
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_KV = 2 * TILE;
-  static constexpr int OFF_SUMS = OFF_KV + SLOTS * TILE;
-  static constexpr int OFF_BAR = OFF_SUMS + (PT_SUMS + 8) * 4;
+  static constexpr int OFF_PLAN = OFF_KV;                // scratch of the count, before the first load
+  static constexpr int OFF_START = OFF_KV + SLOTS * TILE;
+  static constexpr int OFF_CUT = OFF_START + 48;
+  static constexpr int OFF_BAR = OFF_CUT + 32;
   // q_full[2], q_empty[2], kv_full[SLOTS], kv_empty[SLOTS], s_full[2], p_half[2], p_full[2], o_done[2], o_free[2], done
   static constexpr int NBAR = 4 + 2 * SLOTS + 11;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
@@ -773,14 +781,13 @@ struct PromptSmem {
 };
 
 struct PromptBlock {
-  int seq, hk;
   int tok0;                // packed row of the block's first token
   int left;                // tokens of the sequence from there on
   int pos0;                // position of the first token
   int len;                 // tokens in the cache (cut)
   int floor;               // no query of the sequence sees a key before this one
   int lo[2], cnt[2];       // key tiles of the two query tiles
-  int first, last;         // of both: one range (a window reaches back at least to the token itself)
+  int first, tiles;        // of both: one range (a window reaches back at least to the token itself)
 };
 
 // Packed row i of cu_seqlens, inside the rows there are.
@@ -792,26 +799,9 @@ __device__ __forceinline__ int blocks_of(const AttnArgs& a, int seq, int per) {
   const int n = cut_row(a, seq + 1) - cut_row(a, seq);
   return n > 0 ? (n + per - 1) / per : 0;
 }
-
-// Block idx of the numbering (a warp asks together); sums[g]: blocks before sequence g * group.
-__device__ __forceinline__ PromptBlock find_block(const AttnArgs& a, const int* sums, int group, int per, int tpt,
-                                                  int64_t idx) {
-  const int lane = threadIdx.x & 31;
+__device__ __forceinline__ PromptBlock block_at(const AttnArgs& a, int seq, int blk, int tpt) {
   PromptBlock b;
-  const int blk = (int)(idx / a.Hkv);
-  b.hk = (int)(idx - (int64_t)blk * a.Hkv);
-  int lo = 0;
-#pragma unroll
-  for (int step = PT_SUMS / 32; step >= 1; step = step == 1 ? 0 : 1) {
-    const uint32_t below = __ballot_sync(0xffffffffu, (step > 1 || lane < PT_SUMS / 32) && sums[lo + lane * step] <= blk);
-    lo += (31 - __clz(below)) * step;
-  }
-  // the last of the group's sequences whose first block is not behind blk
-  int seq = lo * group, at = sums[lo];
-  for (int n; seq + 1 < a.num_seqs && blk >= at + (n = blocks_of(a, seq, per)); ++seq) at += n;
-  b.seq = seq;
-  const int first = cut_row(a, seq), n = cut_row(a, seq + 1) - first;
-  const int skip = (blk - at) * per;
+  const int first = cut_row(a, seq), n = cut_row(a, seq + 1) - first, skip = blk * 2 * tpt;
   b.tok0 = first + skip;
   b.left = n - skip;
   b.len = cut_length(a, seq);
@@ -825,14 +815,158 @@ __device__ __forceinline__ PromptBlock find_block(const AttnArgs& a, const int* 
     b.cnt[t] = rows > 0 && p1 >= 0 ? p1 / PT_KEYS - b.lo[t] + 1 : 0;
   }
   b.first = b.cnt[0] > 0 ? b.lo[0] : b.lo[1];
-  b.last = b.cnt[1] > 0 ? b.lo[1] + b.cnt[1] - 1 : b.lo[0] + b.cnt[0] - 1;
+  const int end = b.cnt[1] > 0 ? b.lo[1] + b.cnt[1] : b.lo[0] + b.cnt[0];
+  b.tiles = b.cnt[0] + b.cnt[1] > 0 ? end - b.first : 0;
   return b;
+}
+// A block without a key still counts one, so that its rows are written.
+__device__ __forceinline__ int steps_of(const PromptBlock& b) { return PT_OVER + max(b.tiles, 1); }
+
+// A run of steps as parts of blocks: key tiles [b.first, b.first + b.tiles) of block (seq, blk) of
+// key head hk, the two query tiles' ranges cut to them.
+struct PromptRun {
+  int part_seq, part_hk;
+  int seq, blk, hk, at;    // at: step of the block, its first PT_OVER steps are no tiles
+  int64_t left;
+  int tpt;
+  bool first, starts, ends;   // the part is the run's first one, holds its block's first tile, its last one
+  PromptBlock b;
+  bool begun;
+
+  __device__ __forceinline__ bool next(const AttnArgs& a) {
+    first = !begun;
+    while (left > 0) {
+      b = block_at(a, seq, blk, tpt);
+      part_seq = seq;
+      part_hk = hk;
+      const int all = steps_of(b), steps = (int)min((int64_t)(all - at), left);
+      const int tile = max(at - PT_OVER, 0), n = at + steps - PT_OVER - tile;
+      left -= steps;
+      at += steps;
+      const bool done = at == all;
+      if (done) {                                        // the block after it
+        at = 0;
+        ++blk;
+        while (left > 0 && blk >= blocks_of(a, seq, 2 * tpt)) {
+          blk = 0;
+          if (++seq == a.num_seqs) {
+            seq = 0;
+            ++hk;
+          }
+        }
+      }
+      if (n <= 0) continue;
+      starts = tile == 0;
+      ends = done;
+      if (b.tiles > 0) {
+        b.first += tile;
+        b.tiles = n;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int end = min(b.lo[t] + b.cnt[t], b.first + n);
+          b.lo[t] = max(b.lo[t], b.first);
+          b.cnt[t] = max(end - b.lo[t], 0);
+        }
+      }
+      begun = true;
+      return true;
+    }
+    return false;
+  }
+};
+
+// Parts in the workspace: per CTA and slot (0: the run's first part, 1: its last) the two query tiles'
+// O [hd / 4][128 rows] of four columns, then (max, sum, sink logit) [128 rows]; per CTA what the
+// join has to know.
+__host__ __device__ constexpr int64_t prompt_part_floats(int hd) { return (int64_t)2 * PT_ROWS * (hd + 4); }
+struct PromptCut {
+  int cut, cont;           // the run's last part does not end its block; its first one does not start it
+  int single;              // both are the same part
+  int slot, hk, tok0, left, pad;
+};
+
+// Exclusive scan over the PT_PLAN threads of warps 4 .. 11.
+__device__ __forceinline__ int64_t plan_scan(int64_t v, int64_t* s, int64_t* sum) {
+  const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) - 4;
+  int64_t inc = v;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int64_t o = __shfl_up_sync(0xffffffffu, inc, off);
+    if (lane >= off) inc += o;
+  }
+  if (lane == 31) s[warp] = inc;
+  asm volatile("bar.sync 1, 256;" ::: "memory");
+  int64_t before = inc - v, all = 0;
+#pragma unroll
+  for (int w = 0; w < PT_PLAN / 32; ++w) {
+    if (w < warp) before += s[w];
+    all += s[w];
+  }
+  asm volatile("bar.sync 1, 256;" ::: "memory");
+  *sum = all;
+  return before;
+}
+
+// This CTA's run, found by warps 4 .. 11: blocks counted over groups of sequences, steps over groups of blocks.
+__device__ __forceinline__ void plan_run(const AttnArgs& a, int tpt, uint8_t* scratch, PromptRun* out) {
+  int64_t* s = reinterpret_cast<int64_t*>(scratch);
+  int64_t* sums = s + PT_PLAN / 32;                      // blocks before each group
+  const int g = threadIdx.x - 128, per = 2 * tpt;
+  const int group = (a.num_seqs + PT_PLAN - 1) / PT_PLAN;
+  int64_t mine = 0, blocks, steps;
+  for (int q = g * group; q < min(a.num_seqs, (g + 1) * group); ++q) mine += blocks_of(a, q, per);
+  sums[g] = plan_scan(mine, s, &blocks);
+  asm volatile("bar.sync 1, 256;" ::: "memory");
+  const int64_t b0 = blocks * g / PT_PLAN, b1 = blocks * (g + 1) / PT_PLAN;
+  int seq = 0, blk = 0;
+  if (b0 < b1) {                                         // block b0: its group, then its sequence
+    int lo = 0, hi = PT_PLAN;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (sums[mid] <= b0) lo = mid; else hi = mid;
+    }
+    seq = lo * group;
+    int64_t rest = b0 - sums[lo];
+    for (int n; rest >= (n = blocks_of(a, seq, per)); ++seq) rest -= n;
+    blk = (int)rest;
+  }
+  const int seq0 = seq, blk0 = blk;
+  mine = 0;
+  for (int64_t b = b0; b < b1; ++b) {
+    while (blk >= blocks_of(a, seq, per)) ++seq, blk = 0;
+    mine += steps_of(block_at(a, seq, blk++, tpt));
+  }
+  const int64_t before = plan_scan(mine, s, &steps);
+  if (g == 0) out->left = 0;
+  asm volatile("bar.sync 1, 256;" ::: "memory");
+  if (steps == 0) return;                                // no packed row
+  // no run so short that its start and end cost more than it holds, unless blocks are that short
+  const int64_t all = steps * a.Hkv, want = max(all / PT_LEAST, blocks * a.Hkv);
+  const Runs runs(all, (int)min(want, (int64_t)gridDim.x));
+  if (blockIdx.x >= runs.nb) return;
+  const int64_t begin = runs.begin(blockIdx.x);
+  const int64_t hk = quotient(begin, steps), r = begin - hk * steps;
+  if (r < before || r >= before + mine) return;
+  int64_t at = r - before;
+  seq = seq0, blk = blk0;
+  while (true) {
+    while (blk >= blocks_of(a, seq, per)) ++seq, blk = 0;
+    const int n = steps_of(block_at(a, seq, blk, tpt));
+    if (at < n) break;
+    at -= n;
+    ++blk;
+  }
+  out->seq = seq;
+  out->blk = blk;
+  out->hk = (int)hk;
+  out->at = (int)at;
+  out->left = runs.begin(blockIdx.x + 1) - begin;
 }
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(PT_THREADS, 1)
     paged_prompt_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                        const __grid_constant__ CUtensorMap tmV, const AttnArgs a) {
+                        const __grid_constant__ CUtensorMap tmV, const AttnArgs a, float* parts, PromptCut* cuts) {
   using L = PromptSmem<HD>;
   constexpr int SLOTS = L::SLOTS;
   constexpr int ATOMS = HD / 64, ATOM = 128 * 128;       // 128 rows of 128 bytes
@@ -841,7 +975,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
   constexpr uint32_t IDESC_PV = idesc_f16(128, HD, FMT, 0, 1);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  int* sums = reinterpret_cast<int*>(smem + L::OFF_SUMS);
+  PromptRun* s_run = reinterpret_cast<PromptRun*>(smem + L::OFF_START);   // seq .. left of it
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
   uint64_t* q_empty = q_full + 2;
   uint64_t* kv_full = q_empty + 2;
@@ -856,7 +990,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
   volatile int* s_abort = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = a.H / a.Hkv;
-  const int tpt = PT_ROWS / G, per = 2 * tpt;            // tokens of a tile, of a block
+  const int tpt = PT_ROWS / G;                           // tokens of a tile; a block has two
 
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tmQ);
@@ -883,32 +1017,23 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     tmem_alloc(s_tmem, 512);
     tmem_relinquish();
   }
-  // blocks before each group of sequences
-  const int group = (a.num_seqs + PT_SUMS - 1) / PT_SUMS;
-  if (warp >= 4) {                                       // 256 threads, one group each
-    const int g = threadIdx.x - 128;
-    int mine = 0;
-    for (int s = g * group; s < min(a.num_seqs, (g + 1) * group); ++s) mine += blocks_of(a, s, per);
-    int inc = mine;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const int o = __shfl_up_sync(0xffffffffu, inc, off);
-      if (lane >= off) inc += o;
-    }
-    if (lane == 31) sums[PT_SUMS + warp - 4] = inc;
-    asm volatile("bar.sync 1, 256;" ::: "memory");
-    int before = inc - mine;
-    for (int w = 0; w < warp - 4; ++w) before += sums[PT_SUMS + w];
-    sums[g] = before;
-    if (g == PT_SUMS - 1) s_tmem[2] = before + mine;     // blocks of one key head
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the join waits for this grid's end itself
+  if (warp >= 4) {
+    plan_run(a, tpt, smem + L::OFF_PLAN, s_run);
+    fence_proxy_async_smem();                            // the scratch is written by the copy engine next
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
-  const int64_t total = (int64_t)(int)s_tmem[2] * a.Hkv;
-  // all roles walk the same blocks
-#define ZS_EACH_BLOCK(i) for (int64_t i = total - 1 - (int64_t)blockIdx.x; i >= 0; i -= gridDim.x)
+  PromptRun run;                                         // all roles walk the same parts
+  run.seq = s_run->seq;
+  run.blk = s_run->blk;
+  run.hk = s_run->hk;
+  run.at = s_run->at;
+  run.left = s_run->left;
+  run.tpt = tpt;
+  run.begun = false;
 
   if (warp < 4) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PT_REGS_AUX));
@@ -919,9 +1044,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     uint32_t issued = 0, par = 0, q_n[2] = {0, 0};
     int item = 0;
     bool ok = true;
-    ZS_EACH_BLOCK(i) {
-      if (!ok) break;
-      const PromptBlock b = find_block(a, sums, group, per, tpt, i);
+    while (ok && run.next(a)) {
+      const PromptBlock& b = run.b;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         if (!ok || b.cnt[t] == 0) continue;
@@ -931,17 +1055,17 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
           mbar_arrive_expect_tx(&q_full[t], G * tpt * HD * 2);
 #pragma unroll
           for (int at = 0; at < ATOMS; ++at)
-            tma_load_3d(smem + L::OFF_Q + t * L::TILE + at * ATOM, &tmQ, &q_full[t], at * 64, b.hk * G,
+            tma_load_3d(smem + L::OFF_Q + t * L::TILE + at * ATOM, &tmQ, &q_full[t], at * 64, run.part_hk * G,
                         b.tok0 + t * tpt);
         }
         ++q_n[t];
       }
       if (b.cnt[0] + b.cnt[1] == 0) continue;
-      for (int j = b.first; ok && j <= b.last; ++j) {
+      for (int j = b.first; ok && j < b.first + b.tiles; ++j) {
         const int key = j * PT_KEYS + pg * rows;
         int page = (int)a.num_pages;                     // past the pool: TMA fills zeros
         if (lane < boxes && key < b.len && key + rows > b.floor) {
-          page = __ldg(a.block_table + b.seq * a.bt_ld + key / a.page);
+          page = __ldg(a.block_table + run.part_seq * a.bt_ld + key / a.page);
           if ((unsigned)page >= (unsigned)a.num_pages) {
             record_error(ZS_DEVERR_INDEX);
             page = (int)a.num_pages;
@@ -958,7 +1082,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
           __syncwarp();
           if (lane < boxes)
             tma_load_3d(smem + L::OFF_KV + st * L::TILE + atom * ATOM + pg * rows * 128, kv ? &tmV : &tmK, &kv_full[st],
-                        atom * 64, b.hk * a.page + key % a.page, page);
+                        atom * 64, run.part_hk * a.page + key % a.page, page);
           issued |= 1u << st;
           par = (par & ~(1u << st)) | ((uint32_t)((item / SLOTS) & 1) << st);
         }
@@ -982,11 +1106,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     auto ready = [&](int it) -> bool {
       return warp_wait(&kv_full[it % SLOTS], (it / SLOTS) & 1, s_abort, ZS_DEVERR_TIMEOUT_MMA);
     };
-    ZS_EACH_BLOCK(i) {
-      if (!ok) break;
-      const PromptBlock b = find_block(a, sums, group, per, tpt, i);
+    while (ok && run.next(a)) {
+      const PromptBlock& b = run.b;
       if (b.cnt[0] + b.cnt[1] == 0) continue;
-      const int ulo = b.first, uhi = b.last;
+      const int ulo = b.first, uhi = b.first + b.tiles - 1;
       const int end[2] = {b.lo[0] + b.cnt[0], b.lo[1] + b.cnt[1]};
 #pragma unroll
       for (int t = 0; t < 2; ++t)
@@ -1101,14 +1224,24 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     const uint64_t scale2 = attn::pack2(__float_as_uint(a.scale_log2), __float_as_uint(a.scale_log2));
     uint32_t s_n = 0, b_n = 0, q_n = 0;
     bool ok = true;
-    ZS_EACH_BLOCK(i) {
-      if (!ok) break;
-      const PromptBlock b = find_block(a, sums, group, per, tpt, i);
+    PromptCut* cut = reinterpret_cast<PromptCut*>(smem + L::OFF_CUT);   // one thread's: what the join has to know
+    if (threadIdx.x == 128) *cut = PromptCut{0, 0, 0, 0, 0, 0, 0, 0};
+    while (ok && run.next(a)) {
+      const PromptBlock& b = run.b;
+      if (threadIdx.x == 128) {
+        if (run.first) cut->cont = run.starts ? 0 : 1;
+        cut->cut = run.ends ? 0 : 1;
+        cut->single = run.first ? 1 : 0;
+        cut->slot = run.first ? 0 : 1;
+        cut->hk = run.part_hk;
+        cut->tok0 = b.tok0;
+        cut->left = b.left;
+      }
       const int tokens = min(b.left - t * tpt, tpt);     // of the tile
       if (tokens <= 0) continue;
       const bool valid = tr < tokens;
       const int p0 = b.pos0 + t * tpt, p = p0 + tr;      // the tile's first position, the row's
-      const int h = b.hk * G + min(g, G - 1);
+      const int h = run.part_hk * G + min(g, G - 1);
       const int64_t tok = (int64_t)b.tok0 + t * tpt + tr;
       const int n = t == 0 ? b.cnt[0] : b.cnt[1], lo = t == 0 ? b.lo[0] : b.lo[1];
       float m = -INFINITY, l = 0.f;
@@ -1135,6 +1268,16 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
         ++q_n;
         __syncwarp();
         if (lane == 0) mbar_arrive(&q_empty[t]);
+      } else if (a.k_sink != nullptr && valid) {         // its Q is not loaded
+        const T* q = reinterpret_cast<const T*>(a.q) + tok * a.ldq + (int64_t)h * HD;
+        for (int c = 0; c < HD; c += 4) {
+          float f[4], v[4];
+          unpack4<T>(*reinterpret_cast<const uint2*>(q + c), f);
+          load_sink<4>(a, (int64_t)h * HD + c, v);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) z = fmaf(f[e], v[e], z);
+        }
+        z *= a.scale_log2;
       }
       for (int uu = 0; uu < n; ++uu) {
         const int k0 = (lo + uu) * PT_KEYS;
@@ -1218,22 +1361,30 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
         l += (a0 + a1) + (a2 + a3);
       }
       if (!ok) break;
-      float f = 1.f;
-      if (a.k_sink != nullptr) {
-        const float mt = fmaxf(m, z);
-        f = m == -INFINITY ? 0.f : attn::fast_exp2(m - mt);
-        l = l * f + attn::fast_exp2(z - mt);
-        m = mt;
-      }
-      float inv = l > 0.f ? f / l : (l != l ? l : 0.f);
-      if (valid) {
-        inv *= gate_of<T>(a, tok, h);
-        if (a.lse != nullptr)
-          a.lse[tok * a.H + h] = l > 0.f ? (m + log2f(l)) * 0.6931471805599453f : (l != l ? l : -INFINITY);
-      }
+      const bool whole = run.starts && run.ends;
+      float inv = 1.f;
       T* out = reinterpret_cast<T*>(a.o) + (tok * a.H + h) * HD;
-      if (n == 0) {                                      // all before the sequence's first position
-        if (valid)
+      float4* part = reinterpret_cast<float4*>(parts + ((int64_t)blockIdx.x * 2 + (run.first ? 0 : 1)) * prompt_part_floats(HD)) +
+                     t * PT_ROWS * (HD / 4 + 1) + r;
+      if (whole) {
+        float f = 1.f;
+        if (a.k_sink != nullptr) {
+          const float mt = fmaxf(m, z);
+          f = m == -INFINITY ? 0.f : attn::fast_exp2(m - mt);
+          l = l * f + attn::fast_exp2(z - mt);
+          m = mt;
+        }
+        inv = l > 0.f ? f / l : (l != l ? l : 0.f);
+        if (valid) {
+          inv *= gate_of<T>(a, tok, h);
+          if (a.lse != nullptr)
+            a.lse[tok * a.H + h] = l > 0.f ? (m + log2f(l)) * 0.6931471805599453f : (l != l ? l : -INFINITY);
+        }
+      } else {
+        part[PT_ROWS * (HD / 4)] = make_float4(m, l, z, 0.f);
+      }
+      if (n == 0) {                                      // no key for any row of the tile
+        if (valid && whole)
           for (int c = 0; c < HD; c += 8) *reinterpret_cast<uint4*>(out + c) = make_uint4(0, 0, 0, 0);
         continue;
       }
@@ -1248,7 +1399,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
         uint32_t o[32];
         tmem_ld_32x32b_x32(to + c * 32, o);
         tc_wait_ld();
-        if (valid) {
+        if (!whole) {
+#pragma unroll
+          for (int x = 0; x < 8; ++x)
+            part[(c * 8 + x) * PT_ROWS] = make_float4(__uint_as_float(o[x * 4]), __uint_as_float(o[x * 4 + 1]),
+                                                      __uint_as_float(o[x * 4 + 2]), __uint_as_float(o[x * 4 + 3]));
+        } else if (valid) {
           uint4* dst = reinterpret_cast<uint4*>(out + c * 32);
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
@@ -1263,14 +1419,61 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&o_free[t]);
     }
+    if (threadIdx.x == 128) cuts[blockIdx.x] = *cut;
   }
-#undef ZS_EACH_BLOCK
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
     tmem_dealloc(tmem, 512);
+  }
+}
+
+// Block (c, query tile, 32 columns): the block that the cut behind CTA c goes through, unless an
+// earlier cut does too; its parts in the order of the CTAs, a row per thread.
+template <typename T, int HD>
+__global__ void __launch_bounds__(PT_ROWS) paged_prompt_join_kernel(const AttnArgs a, const float* parts,
+                                                                    const PromptCut* cuts, int ctas) {
+  const int c = blockIdx.x, t = blockIdx.y, col = blockIdx.z * 32, r = threadIdx.x;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const PromptCut cut = cuts[c];
+  if (!cut.cut || (cut.single && cut.cont)) return;
+  const int G = a.H / a.Hkv, tpt = PT_ROWS / G, tr = r / G;
+  if (tr >= min(cut.left - t * tpt, tpt)) return;        // no row of the block
+  const int h = cut.hk * G + r - tr * G;
+  const int64_t tok = (int64_t)cut.tok0 + t * tpt + tr;
+  float m = -INFINITY, l = 0.f, z = 0.f, acc[32];
+#pragma unroll
+  for (int e = 0; e < 32; ++e) acc[e] = 0.f;
+  for (int b = c, slot = cut.slot; b < ctas; ++b, slot = 0) {
+    const float4* part = reinterpret_cast<const float4*>(parts + ((int64_t)b * 2 + slot) * prompt_part_floats(HD)) +
+                         t * PT_ROWS * (HD / 4 + 1) + r;
+    const float4 ml = part[PT_ROWS * (HD / 4)];
+    float4 o[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) o[x] = part[(col / 4 + x) * PT_ROWS];
+    z = ml.z;
+    if (ml.x != -INFINITY || ml.y != 0.f) {              // a part in which the row sees no key has no O
+      const float mt = fmaxf(m, ml.x);
+      const float f = m == -INFINITY ? 0.f : exp2f(m - mt), fb = ml.x == -INFINITY ? 1.f : exp2f(ml.x - mt);
+      l = l * f + ml.y * fb;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        acc[x * 4] = acc[x * 4] * f + o[x].x * fb;
+        acc[x * 4 + 1] = acc[x * 4 + 1] * f + o[x].y * fb;
+        acc[x * 4 + 2] = acc[x * 4 + 2] * f + o[x].z * fb;
+        acc[x * 4 + 3] = acc[x * 4 + 3] * f + o[x].w * fb;
+      }
+      m = mt;
+    }
+    if (b > c && !(cuts[b].cut && cuts[b].single)) break;   // it ends here
+  }
+  const float gate = gate_of<T>(a, tok, h);
+#pragma unroll
+  for (int x = 0; x < 8; ++x) {
+    const float v[4] = {acc[x * 4], acc[x * 4 + 1], acc[x * 4 + 2], acc[x * 4 + 3]};
+    finish_row<T, HD>(a, tok, h, col + x * 4, m, l, v, z, gate, col + x == 0);
   }
 }
 
@@ -1398,8 +1601,28 @@ extern "C" int zs_paged_decode_attention(const void* q, int64_t ldq, const void*
                    : launch_decode<__half, 64>(a, dtype, workspace, stream);
 }
 
+// CTAs for as many steps as the packed rows and the tables leave room for.
+static int prompt_ctas(int64_t tokens, int num_seqs, int H, int Hkv, int max_pages, int page, int window) {
+  const int per = 2 * (paged::PT_ROWS / (H / Hkv));
+  const int64_t blocks = (tokens / per + num_seqs) * Hkv;
+  int64_t tiles = ((int64_t)max_pages * page + paged::PT_KEYS - 1) / paged::PT_KEYS;
+  if (window > 0 && ((int64_t)window + per) / paged::PT_KEYS + 2 < tiles) tiles = ((int64_t)window + per) / paged::PT_KEYS + 2;
+  int64_t want = blocks * (tiles + paged::PT_OVER) / paged::PT_LEAST;
+  if (want < blocks) want = blocks;
+  int sms = num_sms();
+  if (sms > paged::PT_MAX_CTAS) sms = paged::PT_MAX_CTAS;
+  return (int)(want < sms ? want : sms);
+}
+
+extern "C" size_t zs_paged_prompt_workspace(int64_t tokens, int num_seqs, int H, int Hkv, int hd, int max_pages,
+                                            int page, int window) {
+  if (tokens < 1 || num_seqs < 1 || Hkv < 1 || H / Hkv < 1 || H / Hkv > paged::PT_ROWS) return 0;
+  const size_t ctas = (size_t)prompt_ctas(tokens, num_seqs, H, Hkv, max_pages, page, window);
+  return ctas * (2 * paged::prompt_part_floats(hd) * 4 + sizeof(paged::PromptCut)) + 512;
+}
+
 template <typename T, int HD>
-static int launch_prompt(const paged::AttnArgs& a, int dtype, cudaStream_t stream) {
+static int launch_prompt(const paged::AttnArgs& a, int dtype, void* workspace, cudaStream_t stream) {
   using L = paged::PromptSmem<HD>;
   const int G = a.H / a.Hkv, tpt = paged::PT_ROWS / G, box = a.page < paged::PT_KEYS ? a.page : paged::PT_KEYS;
   CUtensorMap tq, tk, tv;
@@ -1409,11 +1632,15 @@ static int launch_prompt(const paged::AttnArgs& a, int dtype, cudaStream_t strea
   if (rc != ZS_OK) return rc;
   rc = make_page_tmap(&tv, a.v_pages, dtype, HD, (int64_t)a.Hkv * a.page, a.num_pages, a.page_stride, box);
   if (rc != ZS_OK) return rc;
-  const int64_t most = (a.tokens / (2 * tpt) + a.num_seqs) * a.Hkv;      // blocks that the packed rows can make
-  const int grid = (int)(most < num_sms() ? most : num_sms());
+  const int grid = prompt_ctas(a.tokens, a.num_seqs, a.H, a.Hkv, a.max_pages, a.page, a.window);
+  float* parts = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t(255));
+  paged::PromptCut* cuts = reinterpret_cast<paged::PromptCut*>(parts + grid * 2 * paged::prompt_part_floats(HD));
   ZS_CUDA_TRY(cudaFuncSetAttribute(paged::paged_prompt_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::ALLOC));
-  paged::paged_prompt_kernel<T, HD><<<grid, paged::PT_THREADS, L::ALLOC, stream>>>(tq, tk, tv, a);
+  paged::paged_prompt_kernel<T, HD><<<grid, paged::PT_THREADS, L::ALLOC, stream>>>(tq, tk, tv, a, parts, cuts);
   ZS_CUDA_TRY(cudaGetLastError());
+  if (grid > 1 && (int64_t)a.max_pages * a.page > paged::PT_KEYS)      // else no block has a second tile to cut at
+    return launch_after(paged::paged_prompt_join_kernel<T, HD>, dim3(grid - 1, 2, HD / 32), dim3(paged::PT_ROWS), stream, a,
+                        parts, cuts, grid);
   return ZS_OK;
 }
 
@@ -1422,7 +1649,8 @@ extern "C" int zs_paged_prompt_attention(const void* q, int64_t ldq, const void*
                                          int64_t bt_ld, int max_pages, const int* seq_lens, const int* cu_seqlens,
                                          int num_seqs, int64_t tokens, int H, int Hkv, int hd, int page, int window,
                                          float scale, const void* k_sink, int sink_dtype, const void* gate,
-                                         int64_t ldg, void* o, float* lse, int dtype, void* stream_) {
+                                         int64_t ldg, void* o, float* lse, int dtype, void* workspace,
+                                         size_t workspace_bytes, void* stream_) {
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   ZS_REQUIRE(cu_seqlens, ZS_ERR_ARG);
   paged::AttnArgs a;
@@ -1431,9 +1659,12 @@ extern "C" int zs_paged_prompt_attention(const void* q, int64_t ldq, const void*
                            ldg, o, lse, dtype);
   if (rc != ZS_OK) return rc;
   ZS_REQUIRE(H / Hkv <= paged::PT_ROWS, ZS_ERR_SHAPE);
+  ZS_REQUIRE(workspace, ZS_ERR_WORKSPACE);
   ZS_BIND(q);
+  ZS_REQUIRE(workspace_bytes >= zs_paged_prompt_workspace(tokens, num_seqs, H, Hkv, hd, max_pages, page, window),
+             ZS_ERR_WORKSPACE);
   if (dtype == ZS_BF16)
-    return hd == 128 ? launch_prompt<__nv_bfloat16, 128>(a, dtype, stream)
-                     : launch_prompt<__nv_bfloat16, 64>(a, dtype, stream);
-  return hd == 128 ? launch_prompt<__half, 128>(a, dtype, stream) : launch_prompt<__half, 64>(a, dtype, stream);
+    return hd == 128 ? launch_prompt<__nv_bfloat16, 128>(a, dtype, workspace, stream)
+                     : launch_prompt<__nv_bfloat16, 64>(a, dtype, workspace, stream);
+  return hd == 128 ? launch_prompt<__half, 128>(a, dtype, workspace, stream) : launch_prompt<__half, 64>(a, dtype, workspace, stream);
 }

@@ -223,13 +223,15 @@ def _attention(q, k_pages, v_pages, block_table, seq_lens, cu_seqlens, window, k
     more = (H, Hkv, hd, page, w, scale, Z.ptr(k_sink), sink_dtype, Z.ptr(gate), ldg, o.data_ptr(), Z.ptr(lse),
             _DTYPES[dtype])
     stream = torch._C._cuda_getCurrentRawStream(dev)
-    Z.count(1)
+    Z.count(2)
     if decode:
         size = L.zs_paged_decode_workspace(n, H, Hkv, hd)
         ws = torch.empty(size, dtype=torch.uint8, device=q.device)
         rc = L.zs_paged_decode_attention(*args, n, *more, ws.data_ptr(), size, stream)
     else:
-        rc = L.zs_paged_prompt_attention(*args, cu_seqlens.data_ptr(), n, T, *more, stream)
+        size = L.zs_paged_prompt_workspace(T, n, H, Hkv, hd, m, page, w)
+        ws = torch.empty(size, dtype=torch.uint8, device=q.device)
+        rc = L.zs_paged_prompt_attention(*args, cu_seqlens.data_ptr(), n, T, *more, ws.data_ptr(), size, stream)
     if rc:
         Z.check(rc, "zs_paged_decode_attention" if decode else "zs_paged_prompt_attention")
     return (o, lse) if return_lse else o

@@ -692,10 +692,11 @@ int zs_sparse_rmsprop_step(float* param, int64_t num_rows, int64_t d, int64_t ld
  *   infinity in a value of the sequence may reach every row of the same
  *   sequence; what lies in the pages outside the sequence reaches none.
  *   H / Hkv <= 128.
- * zs_paged_decode_attention: the same for one token per sequence (row s), with
- *   the keys of a sequence split over blocks and joined in a fixed order;
- *   seq_lens[s] == 0 marks an empty slot (o zero).  The workspace holds partial
- *   results of this call only; calls that may overlap need one each.
+ *   Both attentions split long work over thread blocks and join the parts in a
+ *   fixed order; the workspace holds the parts of this call only, so calls that
+ *   may overlap need one each.
+ * zs_paged_decode_attention: the same for one token per sequence (row s);
+ *   seq_lens[s] == 0 marks an empty slot (o zero).
  */
 int zs_paged_append(const void* qkv, int64_t ld, const float* q_weight, const float* k_weight, float eps,
                     const float* cos, const float* sin, int64_t table_ld, int64_t table_rows, int rot, void* k_pages,
@@ -707,7 +708,9 @@ int zs_paged_prompt_attention(const void* q, int64_t ldq, const void* k_pages, c
                               int max_pages, const int* seq_lens, const int* cu_seqlens, int num_seqs, int64_t tokens,
                               int H, int Hkv, int hd, int page, int window, float scale, const void* k_sink,
                               int sink_dtype, const void* gate, int64_t ldg, void* o, float* lse, int dtype,
-                              void* stream);
+                              void* workspace, size_t workspace_bytes, void* stream);
+size_t zs_paged_prompt_workspace(int64_t tokens, int num_seqs, int H, int Hkv, int hd, int max_pages, int page,
+                                 int window);
 size_t zs_paged_decode_workspace(int num_seqs, int H, int Hkv, int hd);
 int zs_paged_decode_attention(const void* q, int64_t ldq, const void* k_pages, const void* v_pages,
                               int64_t page_stride, int64_t num_pages, const int* block_table, int64_t bt_ld,

@@ -60,7 +60,7 @@ def test_entry_points_refuse_before_the_device(kw, code):
     build.build()
     L = _lib.lib()
     args = _attn_args(**kw)
-    assert L.zs_paged_prompt_attention(*args, None) == code
+    assert L.zs_paged_prompt_attention(*args, 1 << 28, 1 << 40, None) == code
     if "cu" not in kw and "tokens" not in kw:
         d = args[:10] + [args[11]] + args[13:]
         assert L.zs_paged_decode_attention(*d, 1 << 28, 1 << 40, None) == code
@@ -72,7 +72,7 @@ def test_entry_points_refuse_before_the_device(kw, code):
                                  a["tokens"], a["H"], a["Hkv"], a["hd"], a["page"], 1 << 26, args[-1], None) == code
 
 
-def test_decode_refuses_a_missing_workspace():
+def test_attention_refuses_a_missing_workspace():
     from zs_b200 import _lib
 
     L = _lib.lib()
@@ -80,6 +80,8 @@ def test_decode_refuses_a_missing_workspace():
     d = args[:10] + [args[11]] + args[13:]
     assert L.zs_paged_decode_attention(*d, None, 1 << 40, None) == 6
     assert L.zs_paged_decode_attention(*d, 1 << 28, 0, None) == 6
+    assert L.zs_paged_prompt_attention(*args, None, 1 << 40, None) == 6
+    assert L.zs_paged_prompt_workspace(5, 2, 8, 2, 64, 3, 16, 0) > 0
 
 
 @pytest.mark.parametrize("kw,code", [(dict(kv=None), 1), (dict(num_pages=0), 2), (dict(num_pages=2000001), 2),
