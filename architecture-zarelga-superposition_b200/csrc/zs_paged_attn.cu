@@ -30,8 +30,7 @@ struct AttnArgs {
   int H, Hkv, page;
   int window;                  // 0: none
   float scale, scale_log2;
-  const void* k_sink;          // nullable [H, hd]
-  int sink_dtype;
+  const float* k_sink;         // nullable [H, hd]
   const void* gate;            // nullable [tokens, H] rows of ldg elements
   int64_t ldg;
   void* o;                     // [tokens, H, hd] packed
@@ -146,25 +145,6 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, u
       : "memory");
 }
 
-// N consecutive values of the sink from element i (a multiple of N).
-template <int N>
-__device__ __forceinline__ void load_sink(const AttnArgs& a, int64_t i, float (&v)[N]) {
-  static_assert(N == 4, "4 values a lane");
-  if (a.sink_dtype == ZS_F32) {
-    const float4 x = __ldg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(a.k_sink) + i));
-    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
-  } else {
-    const uint2 x = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(a.k_sink) + i));
-    const uint32_t w[2] = {x.x, x.y};
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const float2 f = a.sink_dtype == ZS_BF16 ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[e]))
-                                               : __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
-      v[2 * e] = f.x, v[2 * e + 1] = f.y;
-    }
-  }
-}
-
 // The sink's logit of query head h (log2 units), summed over LANES neighbouring lanes that call
 // together (all of the warp's lanes call).
 template <typename T, int HD, int LANES>
@@ -177,12 +157,11 @@ __device__ __forceinline__ float sink_logit(const AttnArgs& a, int64_t tok, int 
     const uint2 x = *reinterpret_cast<const uint2*>(q + c);
     const float2 f0 = Pair<T>::to_f(*reinterpret_cast<const typename Pair<T>::type*>(&x.x));
     const float2 f1 = Pair<T>::to_f(*reinterpret_cast<const typename Pair<T>::type*>(&x.y));
-    float v[4];
-    load_sink<4>(a, (int64_t)h * HD + c, v);
-    dot = fmaf(f0.x, v[0], dot);
-    dot = fmaf(f0.y, v[1], dot);
-    dot = fmaf(f1.x, v[2], dot);
-    dot = fmaf(f1.y, v[3], dot);
+    const float4 v = __ldg(reinterpret_cast<const float4*>(a.k_sink + (int64_t)h * HD + c));
+    dot = fmaf(f0.x, v.x, dot);
+    dot = fmaf(f0.y, v.y, dot);
+    dot = fmaf(f1.x, v.z, dot);
+    dot = fmaf(f1.y, v.w, dot);
   }
 #pragma unroll
   for (int off = LANES / 2; off > 0; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
@@ -770,11 +749,13 @@ struct PromptSmem {
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_KV = 2 * TILE;
   static constexpr int OFF_PLAN = OFF_KV;                // scratch of the count, before the first load
-  static constexpr int OFF_START = OFF_KV + SLOTS * TILE;
-  static constexpr int OFF_CUT = OFF_START + 48;
-  static constexpr int OFF_BAR = OFF_CUT + 32;
-  // q_full[2], q_empty[2], kv_full[SLOTS], kv_empty[SLOTS], s_full[2], p_half[2], p_full[2], o_done[2], o_free[2], done
-  static constexpr int NBAR = 4 + 2 * SLOTS + 11;
+  static constexpr int OFF_PART = OFF_KV + SLOTS * TILE; // parts published by the loading warp (64 bytes each)
+  static constexpr int OFF_CUT = OFF_PART + 4 * 64;
+  static constexpr int OFF_Z = OFF_CUT + 32;             // sink logits of the query tiles' rows
+  static constexpr int OFF_BAR = OFF_Z + 2 * 128 * 4;
+  // q_full[2], q_empty[2], kv_full[SLOTS], kv_empty[SLOTS], s_full[2], p_half[2], p_full[2], o_done[2], o_free[2],
+  // z_full[2], z_free[2], part_full[4], part_empty[4], done
+  static constexpr int NBAR = 4 + 2 * SLOTS + 23;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int TOTAL = OFF_MISC + 16;
   static constexpr int ALLOC = TOTAL + 1024;
@@ -874,6 +855,15 @@ struct PromptRun {
     return false;
   }
 };
+
+// A part as the loading warp publishes it to the others.
+struct PromptPart {
+  int live;                // 0: the run has ended
+  int hk, tok0, left, pos0, len, floor;
+  int lo[2], cnt[2], first, tiles;
+  int flags;               // 1: the run's first part, 2: holds its block's first tile, 4: its last one
+};
+constexpr int PT_PARTS = 4;
 
 // Parts in the workspace: per CTA and slot (0: the run's first part, 1: its last) the two query tiles'
 // O [hd / 4][128 rows] of four columns, then (max, sum, sink logit) [128 rows]; per CTA what the
@@ -975,7 +965,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
   constexpr uint32_t IDESC_PV = idesc_f16(128, HD, FMT, 0, 1);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  PromptRun* s_run = reinterpret_cast<PromptRun*>(smem + L::OFF_START);   // seq .. left of it
+  PromptRun* s_run = reinterpret_cast<PromptRun*>(smem + L::OFF_PART);    // seq .. left of it, before the first part
+  PromptPart* s_part = reinterpret_cast<PromptPart*>(smem + L::OFF_PART);
+  float* s_z = reinterpret_cast<float*>(smem + L::OFF_Z);
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
   uint64_t* q_empty = q_full + 2;
   uint64_t* kv_full = q_empty + 2;
@@ -985,7 +977,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
   uint64_t* p_full = p_half + 2;
   uint64_t* o_done = p_full + 2;
   uint64_t* o_free = o_done + 2;
-  uint64_t* done = o_free + 2;
+  uint64_t* z_full = o_free + 2;
+  uint64_t* z_free = z_full + 2;
+  uint64_t* part_full = z_free + 2;
+  uint64_t* part_empty = part_full + PT_PARTS;
+  uint64_t* done = part_empty + PT_PARTS;
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
   volatile int* s_abort = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -998,16 +994,22 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     tma_prefetch_desc(&tmV);
     for (int t = 0; t < 2; ++t) {
       mbar_init(&q_full[t], 1);
-      mbar_init(&q_empty[t], 5);                         // its last product, and the softmax warps
+      mbar_init(&q_empty[t], 2);                         // its last product, and its sink logits
       mbar_init(&s_full[t], 1);
       mbar_init(&p_half[t], 4);
       mbar_init(&p_full[t], 4);
       mbar_init(&o_done[t], 1);
       mbar_init(&o_free[t], 4);
+      mbar_init(&z_full[t], 1);
+      mbar_init(&z_free[t], 4);
     }
     for (int s = 0; s < SLOTS; ++s) {
       mbar_init(&kv_full[s], 1);
       mbar_init(&kv_empty[s], 1);
+    }
+    for (int s = 0; s < PT_PARTS; ++s) {
+      mbar_init(&part_full[s], 1);
+      mbar_init(&part_empty[s], 11);                     // products, sink logits, softmax
     }
     mbar_init(done, 1);
     *s_abort = 0;
@@ -1026,14 +1028,17 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
-  PromptRun run;                                         // all roles walk the same parts
-  run.seq = s_run->seq;
-  run.blk = s_run->blk;
-  run.hk = s_run->hk;
-  run.at = s_run->at;
-  run.left = s_run->left;
-  run.tpt = tpt;
-  run.begun = false;
+  // The next part, for a warp other than the loading one.
+  uint32_t part_n = 0;
+  auto next_part = [&](PromptPart& b) -> bool {
+    const int sl = part_n % PT_PARTS;
+    if (!warp_wait(&part_full[sl], part_n / PT_PARTS & 1, s_abort, ZS_DEVERR_TIMEOUT_PRODUCER)) return false;
+    b = s_part[sl];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&part_empty[sl]);
+    ++part_n;
+    return b.live != 0;
+  };
 
   if (warp < 4) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PT_REGS_AUX));
@@ -1044,8 +1049,41 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     uint32_t issued = 0, par = 0, q_n[2] = {0, 0};
     int item = 0;
     bool ok = true;
-    while (ok && run.next(a)) {
+    PromptRun run;
+    run.seq = s_run->seq;
+    run.blk = s_run->blk;
+    run.hk = s_run->hk;
+    run.at = s_run->at;
+    run.left = s_run->left;
+    run.tpt = tpt;
+    run.begun = false;
+    __syncwarp();
+    while (ok) {
+      const bool live = run.next(a);
       const PromptBlock& b = run.b;
+      const int sl = part_n % PT_PARTS;
+      ok = warp_wait(&part_empty[sl], part_n / PT_PARTS & 1 ^ 1, s_abort, ZS_DEVERR_TIMEOUT_PRODUCER);
+      if (!ok) break;
+      if (lane == 0) {
+        PromptPart& o = s_part[sl];
+        o.live = live ? 1 : 0;
+        o.hk = run.part_hk;
+        o.tok0 = b.tok0;
+        o.left = b.left;
+        o.pos0 = b.pos0;
+        o.len = b.len;
+        o.floor = b.floor;
+        o.lo[0] = b.lo[0];
+        o.lo[1] = b.lo[1];
+        o.cnt[0] = b.cnt[0];
+        o.cnt[1] = b.cnt[1];
+        o.first = b.first;
+        o.tiles = b.tiles;
+        o.flags = (run.first ? 1 : 0) | (run.starts ? 2 : 0) | (run.ends ? 4 : 0);
+        mbar_arrive(&part_full[sl]);
+      }
+      ++part_n;
+      if (!live) break;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         if (!ok || b.cnt[t] == 0) continue;
@@ -1106,8 +1144,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     auto ready = [&](int it) -> bool {
       return warp_wait(&kv_full[it % SLOTS], (it / SLOTS) & 1, s_abort, ZS_DEVERR_TIMEOUT_MMA);
     };
-    while (ok && run.next(a)) {
-      const PromptBlock& b = run.b;
+    PromptPart b;
+    while (ok && next_part(b)) {
       if (b.cnt[0] + b.cnt[1] == 0) continue;
       const int ulo = b.first, uhi = b.first + b.tiles - 1;
       const int end[2] = {b.lo[0] + b.cnt[0], b.lo[1] + b.cnt[1]};
@@ -1198,7 +1236,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
       __syncwarp();
     }
   } else {
-    // ------------------------------------------------------------------ rows of no sequence
+    // ------------------------------------------------------------------ rows of no sequence, sink logits of tile t
+    const int t = warp - 2;
     const int64_t end = cut_row(a, a.num_seqs), begin = cut_row(a, 0);
     const int64_t me = (int64_t)blockIdx.x * 64 + threadIdx.x - 64, all = (int64_t)gridDim.x * 64;
     const int64_t words = (int64_t)a.H * (HD / 8);
@@ -1211,6 +1250,57 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
       reinterpret_cast<uint4*>(a.o)[e] = make_uint4(0, 0, 0, 0);
       if (a.lse != nullptr && e % (HD / 8) == 0) a.lse[e / (HD / 8)] = -INFINITY;
     }
+    __syncwarp();
+    uint32_t q_n = 0, z_n = 0;
+    bool ok = true;
+    PromptPart b;
+    while (ok && next_part(b)) {
+      const int tokens = min(b.left - t * tpt, tpt);
+      if (tokens <= 0) continue;
+      const bool loaded = (t == 0 ? b.cnt[0] : b.cnt[1]) > 0;
+      if (loaded) ok = warp_wait(&q_full[t], q_n++ & 1, s_abort, ZS_DEVERR_TIMEOUT_EPILOGUE);
+      if (!ok) break;
+      if (a.k_sink != nullptr && loaded) {
+        // Head by head, a row's columns over the lanes, from the Q tile (swizzled 16-byte chunks); the
+        // next head's sink (from L2) is asked for ahead.  Little code and no division: what runs once a
+        // part is fetched anew each time.
+        const int col = lane * 4 & (HD - 1);
+        const uint8_t* qt = smem + L::OFF_Q + t * L::TILE + (col >> 6) * ATOM + (col & 4) * 2;
+        const float* sink = a.k_sink + (int64_t)b.hk * G * HD + col;
+        float4 w = __ldg(reinterpret_cast<const float4*>(sink));
+        ok = warp_wait(&z_free[t], (z_n++ & 1) ^ 1, s_abort, ZS_DEVERR_TIMEOUT_EPILOGUE);
+        if (!ok) break;
+#pragma unroll 1
+        for (int g = 0; g < G; ++g) {
+          const float4 ahead = __ldg(reinterpret_cast<const float4*>(sink + (int64_t)min(g + 1, G - 1) * HD));
+#pragma unroll 1
+          for (int tr = 0; tr < tokens; tr += 8) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int row = min(tr + i, tokens - 1) * G + g;
+              float f[4];
+              unpack4<T>(*reinterpret_cast<const uint2*>(qt + row * 128 + (((col >> 3 & 7) ^ (row & 7)) << 4)), f);
+              v[i] = f[0] * w.x + f[1] * w.y + f[2] * w.z + f[3] * w.w;
+            }
+#pragma unroll
+            for (int off = HD / 8; off > 0; off >>= 1)
+#pragma unroll
+              for (int i = 0; i < 8; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], off);
+            if (lane == 0) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                if (tr + i < tokens) s_z[t * PT_ROWS + (tr + i) * G + g] = v[i];
+            }
+          }
+          w = ahead;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&z_full[t]);
+      }
+      __syncwarp();
+      if (loaded && lane == 0) mbar_arrive(&q_empty[t]);
+    }
   }
   } else {
     // ------------------------------------------------------------------ softmax
@@ -1222,18 +1312,18 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const uint32_t ts = tmem + lane_base + t * 128, to = tmem + lane_base + 256 + t * HD;
     const uint64_t scale2 = attn::pack2(__float_as_uint(a.scale_log2), __float_as_uint(a.scale_log2));
-    uint32_t s_n = 0, b_n = 0, q_n = 0;
+    uint32_t s_n = 0, b_n = 0, z_n = 0;
     bool ok = true;
     PromptCut* cut = reinterpret_cast<PromptCut*>(smem + L::OFF_CUT);   // one thread's: what the join has to know
     if (threadIdx.x == 128) *cut = PromptCut{0, 0, 0, 0, 0, 0, 0, 0};
-    while (ok && run.next(a)) {
-      const PromptBlock& b = run.b;
+    PromptPart b;
+    while (ok && next_part(b)) {
       if (threadIdx.x == 128) {
-        if (run.first) cut->cont = run.starts ? 0 : 1;
-        cut->cut = run.ends ? 0 : 1;
-        cut->single = run.first ? 1 : 0;
-        cut->slot = run.first ? 0 : 1;
-        cut->hk = run.part_hk;
+        if (b.flags & 1) cut->cont = b.flags & 2 ? 0 : 1;
+        cut->cut = b.flags & 4 ? 0 : 1;
+        cut->single = b.flags & 1;
+        cut->slot = b.flags & 1 ? 0 : 1;
+        cut->hk = b.hk;
         cut->tok0 = b.tok0;
         cut->left = b.left;
       }
@@ -1241,44 +1331,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
       if (tokens <= 0) continue;
       const bool valid = tr < tokens;
       const int p0 = b.pos0 + t * tpt, p = p0 + tr;      // the tile's first position, the row's
-      const int h = run.part_hk * G + min(g, G - 1);
+      const int h = b.hk * G + g;
       const int64_t tok = (int64_t)b.tok0 + t * tpt + tr;
+      const float gate = valid ? gate_of<T>(a, tok, h) : 1.f;   // asked for here, used when the part ends
       const int n = t == 0 ? b.cnt[0] : b.cnt[1], lo = t == 0 ? b.lo[0] : b.lo[1];
       float m = -INFINITY, l = 0.f;
-      float z = 0.f;
-      if (n > 0) {
-        if (a.k_sink != nullptr) {                       // the row's sink logit, from the Q tile (swizzled 16-byte chunks)
-          if (!warp_wait(&q_full[t], q_n & 1, s_abort, ZS_DEVERR_TIMEOUT_EPILOGUE)) {
-            ok = false;
-            break;
-          }
-          const uint8_t* qrow = smem + L::OFF_Q + t * L::TILE + r * 128;
-#pragma unroll 4
-          for (int ch = 0; ch < HD / 8; ++ch) {
-            const uint4 x = *reinterpret_cast<const uint4*>(qrow + (ch >> 3) * ATOM + (((ch & 7) ^ (r & 7)) << 4));
-            float f[8], v[8];
-            unpack8<T>(x, f);
-            load_sink<4>(a, (int64_t)h * HD + ch * 8, *reinterpret_cast<float(*)[4]>(v));
-            load_sink<4>(a, (int64_t)h * HD + ch * 8 + 4, *reinterpret_cast<float(*)[4]>(v + 4));
-#pragma unroll
-            for (int e = 0; e < 8; ++e) z = fmaf(f[e], v[e], z);
-          }
-          z *= a.scale_log2;
-        }
-        ++q_n;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&q_empty[t]);
-      } else if (a.k_sink != nullptr && valid) {         // its Q is not loaded
-        const T* q = reinterpret_cast<const T*>(a.q) + tok * a.ldq + (int64_t)h * HD;
-        for (int c = 0; c < HD; c += 4) {
-          float f[4], v[4];
-          unpack4<T>(*reinterpret_cast<const uint2*>(q + c), f);
-          load_sink<4>(a, (int64_t)h * HD + c, v);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) z = fmaf(f[e], v[e], z);
-        }
-        z *= a.scale_log2;
-      }
       for (int uu = 0; uu < n; ++uu) {
         const int k0 = (lo + uu) * PT_KEYS;
         if (!warp_wait(&s_full[t], s_n & 1, s_abort, ZS_DEVERR_TIMEOUT_EPILOGUE)) {
@@ -1361,10 +1418,27 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
         l += (a0 + a1) + (a2 + a3);
       }
       if (!ok) break;
-      const bool whole = run.starts && run.ends;
+      float z = 0.f;
+      if (a.k_sink != nullptr && n == 0) {               // its Q is not loaded
+        if (valid) {
+          const T* q = reinterpret_cast<const T*>(a.q) + tok * a.ldq + (int64_t)h * HD;
+#pragma unroll 1
+          for (int c = 0; c < HD; ++c) z = fmaf(to_f32(q[c]), __ldg(a.k_sink + (int64_t)h * HD + c), z);
+          z *= a.scale_log2;
+        }
+      } else if (a.k_sink != nullptr) {
+        if (!warp_wait(&z_full[t], z_n++ & 1, s_abort, ZS_DEVERR_TIMEOUT_EPILOGUE)) {
+          ok = false;
+          break;
+        }
+        z = s_z[t * PT_ROWS + r] * a.scale_log2;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&z_free[t]);
+      }
+      const bool whole = (b.flags & 6) == 6;
       float inv = 1.f;
       T* out = reinterpret_cast<T*>(a.o) + (tok * a.H + h) * HD;
-      float4* part = reinterpret_cast<float4*>(parts + ((int64_t)blockIdx.x * 2 + (run.first ? 0 : 1)) * prompt_part_floats(HD)) +
+      float4* part = reinterpret_cast<float4*>(parts + ((int64_t)blockIdx.x * 2 + (b.flags & 1 ? 0 : 1)) * prompt_part_floats(HD)) +
                      t * PT_ROWS * (HD / 4 + 1) + r;
       if (whole) {
         float f = 1.f;
@@ -1376,7 +1450,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
         }
         inv = l > 0.f ? f / l : (l != l ? l : 0.f);
         if (valid) {
-          inv *= gate_of<T>(a, tok, h);
+          inv *= gate;
           if (a.lse != nullptr)
             a.lse[tok * a.H + h] = l > 0.f ? (m + log2f(l)) * 0.6931471805599453f : (l != l ? l : -INFINITY);
         }
@@ -1485,7 +1559,7 @@ using namespace zs;
 static int attn_args(paged::AttnArgs& a, const void* q, int64_t ldq, const void* k_pages, const void* v_pages,
                      int64_t page_stride, int64_t num_pages, const int* block_table, int64_t bt_ld, int max_pages,
                      const int* seq_lens, const int* cu, int num_seqs, int64_t tokens, int H, int Hkv, int hd, int page,
-                     int window, float scale, const void* k_sink, int sink_dtype, const void* gate, int64_t ldg,
+                     int window, float scale, const float* k_sink, const void* gate, int64_t ldg,
                      void* o, float* lse, int dtype) {
   const int rc = pages_ok(k_pages, v_pages, page_stride, num_pages, block_table, bt_ld, max_pages, seq_lens, num_seqs,
                           tokens, H, Hkv, hd, page, dtype);
@@ -1493,7 +1567,6 @@ static int attn_args(paged::AttnArgs& a, const void* q, int64_t ldq, const void*
   ZS_REQUIRE(q && o, ZS_ERR_ARG);
   ZS_REQUIRE(window >= 0 && ldq >= (int64_t)H * hd && (gate == nullptr || ldg >= H), ZS_ERR_SHAPE);
   ZS_REQUIRE(ldq % 8 == 0 && ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(o)) & 15) == 0, ZS_ERR_ALIGN);
-  ZS_REQUIRE(k_sink == nullptr || sink_dtype == ZS_F32 || sink_dtype == ZS_BF16 || sink_dtype == ZS_F16, ZS_ERR_DTYPE);
   ZS_REQUIRE((reinterpret_cast<uintptr_t>(k_sink) & 15) == 0, ZS_ERR_ALIGN);
   a.q = q;
   a.ldq = ldq;
@@ -1515,7 +1588,6 @@ static int attn_args(paged::AttnArgs& a, const void* q, int64_t ldq, const void*
   a.scale = scale;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.k_sink = k_sink;
-  a.sink_dtype = sink_dtype;
   a.gate = gate;
   a.ldg = ldg;
   a.o = o;
@@ -1583,13 +1655,13 @@ extern "C" size_t zs_paged_decode_workspace(int num_seqs, int H, int Hkv, int hd
 extern "C" int zs_paged_decode_attention(const void* q, int64_t ldq, const void* k_pages, const void* v_pages,
                                          int64_t page_stride, int64_t num_pages, const int* block_table,
                                          int64_t bt_ld, int max_pages, const int* seq_lens, int num_seqs, int H,
-                                         int Hkv, int hd, int page, int window, float scale, const void* k_sink,
-                                         int sink_dtype, const void* gate, int64_t ldg, void* o, float* lse, int dtype,
+                                         int Hkv, int hd, int page, int window, float scale, const float* k_sink,
+                                         const void* gate, int64_t ldg, void* o, float* lse, int dtype,
                                          void* workspace, size_t workspace_bytes, void* stream_) {
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   paged::AttnArgs a;
   const int rc = attn_args(a, q, ldq, k_pages, v_pages, page_stride, num_pages, block_table, bt_ld, max_pages, seq_lens,
-                           nullptr, num_seqs, num_seqs, H, Hkv, hd, page, window, scale, k_sink, sink_dtype, gate, ldg,
+                           nullptr, num_seqs, num_seqs, H, Hkv, hd, page, window, scale, k_sink, gate, ldg,
                            o, lse, dtype);
   if (rc != ZS_OK) return rc;
   ZS_REQUIRE(workspace && workspace_bytes >= zs_paged_decode_workspace(num_seqs, H, Hkv, hd), ZS_ERR_WORKSPACE);
@@ -1648,14 +1720,14 @@ extern "C" int zs_paged_prompt_attention(const void* q, int64_t ldq, const void*
                                          int64_t page_stride, int64_t num_pages, const int* block_table,
                                          int64_t bt_ld, int max_pages, const int* seq_lens, const int* cu_seqlens,
                                          int num_seqs, int64_t tokens, int H, int Hkv, int hd, int page, int window,
-                                         float scale, const void* k_sink, int sink_dtype, const void* gate,
+                                         float scale, const float* k_sink, const void* gate,
                                          int64_t ldg, void* o, float* lse, int dtype, void* workspace,
                                          size_t workspace_bytes, void* stream_) {
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   ZS_REQUIRE(cu_seqlens, ZS_ERR_ARG);
   paged::AttnArgs a;
   const int rc = attn_args(a, q, ldq, k_pages, v_pages, page_stride, num_pages, block_table, bt_ld, max_pages, seq_lens,
-                           cu_seqlens, num_seqs, tokens, H, Hkv, hd, page, window, scale, k_sink, sink_dtype, gate,
+                           cu_seqlens, num_seqs, tokens, H, Hkv, hd, page, window, scale, k_sink, gate,
                            ldg, o, lse, dtype);
   if (rc != ZS_OK) return rc;
   ZS_REQUIRE(H / Hkv <= paged::PT_ROWS, ZS_ERR_SHAPE);

@@ -121,12 +121,12 @@ _SIGNATURES = {
     "zs_paged_append": (_i32, [_vp, _i64, _vp, _vp, _f32, _vp, _vp, _i64, _i64, _i32, _vp, _vp, _i64, _i64, _vp, _i64,
                                _i32, _vp, _vp, _i32, _i64, _i32, _i32, _i32, _i32, _vp, _i32, _vp]),
     "zs_paged_prompt_attention": (_i32, [_vp, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i32, _vp, _vp, _i32, _i64, _i32,
-                                         _i32, _i32, _i32, _i32, _f32, _vp, _i32, _vp, _i64, _vp, _vp, _i32, _vp, _sz,
+                                         _i32, _i32, _i32, _i32, _f32, _vp, _vp, _i64, _vp, _vp, _i32, _vp, _sz,
                                          _vp]),
     "zs_paged_prompt_workspace": (_sz, [_i64] + [_i32] * 7),
     "zs_paged_decode_workspace": (_sz, [_i32, _i32, _i32, _i32]),
     "zs_paged_decode_attention": (_i32, [_vp, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i32, _vp, _i32, _i32, _i32, _i32,
-                                         _i32, _i32, _f32, _vp, _i32, _vp, _i64, _vp, _vp, _i32, _vp, _sz, _vp]),
+                                         _i32, _i32, _f32, _vp, _vp, _i64, _vp, _vp, _i32, _vp, _sz, _vp]),
     "zs_kv_workspace": (_sz, [ctypes.POINTER(KvCache), _i64]),
     "zs_kv_extend": (_i32, [ctypes.POINTER(KvCache), _vp, _vp, _i64, _vp, _sz, _vp]),
     "zs_kv_fork": (_i32, [ctypes.POINTER(KvCache), _vp, _vp, _i64, _vp, _sz, _vp]),

@@ -188,15 +188,11 @@ def _attention(q, k_pages, v_pages, block_table, seq_lens, cu_seqlens, window, k
         w = int(window)
         if w <= 0 or w >= 1 << 31:
             _fail(f"window must be None or positive (got {window!r})")
-    sink_dtype = 0
     if k_sink is not None:
-        if k_sink.shape != (H, hd):
-            _fail(f"k_sink must be [{H}, {hd}] (got {tuple(k_sink.shape)})")
-        if not k_sink.is_contiguous():
-            k_sink = k_sink.contiguous()
-        if k_sink.data_ptr() % 16:
-            k_sink = k_sink.clone()
-        sink_dtype = Z.dtype_code(k_sink.dtype)
+        if k_sink.shape != (H, hd) or not k_sink.is_floating_point():
+            _fail(f"k_sink must be a floating-point [{H}, {hd}] (got {k_sink.dtype} {tuple(k_sink.shape)})")
+        if k_sink.dtype != torch.float32 or not k_sink.is_contiguous() or k_sink.data_ptr() % 16:
+            k_sink = k_sink.to(torch.float32, copy=True, memory_format=torch.contiguous_format)
     ldg = 0
     if gate is not None:
         if gate.shape != (T, H) or gate.dtype != dtype:
@@ -220,7 +216,7 @@ def _attention(q, k_pages, v_pages, block_table, seq_lens, cu_seqlens, window, k
     L = Z.lib()
     args = (x, max(ldq, H * hd), k_pages.data_ptr(), v_pages.data_ptr(), stride, P, block_table.data_ptr(), bt_ld, m,
             seq_lens.data_ptr())
-    more = (H, Hkv, hd, page, w, scale, Z.ptr(k_sink), sink_dtype, Z.ptr(gate), ldg, o.data_ptr(), Z.ptr(lse),
+    more = (H, Hkv, hd, page, w, scale, Z.ptr(k_sink), Z.ptr(gate), ldg, o.data_ptr(), Z.ptr(lse),
             _DTYPES[dtype])
     stream = torch._C._cuda_getCurrentRawStream(dev)
     Z.count(2)

@@ -684,8 +684,8 @@ int zs_sparse_rmsprop_step(float* param, int64_t num_rows, int64_t d, int64_t ld
  *   nothing is stored.
  * zs_paged_prompt_attention: o[t, h] = sum_k softmax_k(scale q[t, h] . K_k) V_k
  *   over the keys k <= p of row t's sequence (p its position; p - k < window when
- *   window > 0), key head h / (H / Hkv); k_sink [H, hd] (nullable): one more
- *   logit scale q . k_sink whose value is zero; gate (nullable, q's dtype, rows
+ *   window > 0), key head h / (H / Hkv); k_sink f32 [H, hd] (nullable): one
+ *   more logit scale q . k_sink whose value is zero; gate (nullable, q's dtype, rows
  *   of ldg): o is multiplied by sigmoid(gate[t, h]).  lse (nullable) f32
  *   [tokens, H]: the log-sum-exp, sink included.  Padding and rows that see no
  *   key: o is zero (lse of padding outside every sequence: -inf).  A NaN or
@@ -706,8 +706,8 @@ int zs_paged_append(const void* qkv, int64_t ld, const float* q_weight, const fl
 int zs_paged_prompt_attention(const void* q, int64_t ldq, const void* k_pages, const void* v_pages,
                               int64_t page_stride, int64_t num_pages, const int* block_table, int64_t bt_ld,
                               int max_pages, const int* seq_lens, const int* cu_seqlens, int num_seqs, int64_t tokens,
-                              int H, int Hkv, int hd, int page, int window, float scale, const void* k_sink,
-                              int sink_dtype, const void* gate, int64_t ldg, void* o, float* lse, int dtype,
+                              int H, int Hkv, int hd, int page, int window, float scale, const float* k_sink,
+                              const void* gate, int64_t ldg, void* o, float* lse, int dtype,
                               void* workspace, size_t workspace_bytes, void* stream);
 size_t zs_paged_prompt_workspace(int64_t tokens, int num_seqs, int H, int Hkv, int hd, int max_pages, int page,
                                  int window);
@@ -715,9 +715,8 @@ size_t zs_paged_decode_workspace(int num_seqs, int H, int Hkv, int hd);
 int zs_paged_decode_attention(const void* q, int64_t ldq, const void* k_pages, const void* v_pages,
                               int64_t page_stride, int64_t num_pages, const int* block_table, int64_t bt_ld,
                               int max_pages, const int* seq_lens, int num_seqs, int H, int Hkv, int hd, int page,
-                              int window, float scale, const void* k_sink, int sink_dtype, const void* gate,
-                              int64_t ldg, void* o, float* lse, int dtype, void* workspace, size_t workspace_bytes,
-                              void* stream);
+                              int window, float scale, const float* k_sink, const void* gate, int64_t ldg, void* o,
+                              float* lse, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * The cache's bookkeeping, on the device: kv [n_layers, 2, num_pages,

@@ -43,7 +43,7 @@ def _attn_args(**kw):
     # numbers in place of pointers: a refused call reads none of them
     a = dict(q=1 << 20, ldq=512, k=1 << 21, v=1 << 22, stride=2 * 16 * 64, pages=4, table=1 << 23, bt_ld=3, max_pages=3,
              lens=1 << 24, cu=1 << 25, n=2, tokens=5, H=8, Hkv=2, hd=64, page=16, window=0, scale=0.1, sink=None,
-             sink_dt=0, gate=None, ldg=0, o=1 << 26, lse=None, dtype=1)
+             gate=None, ldg=0, o=1 << 26, lse=None, dtype=1)
     a.update(kw)
     return list(a.values())
 
@@ -52,7 +52,7 @@ def _attn_args(**kw):
     (dict(q=None), 1), (dict(o=None), 1), (dict(table=None), 1), (dict(cu=None), 1), (dict(dtype=0), 3),
     (dict(hd=96), 2), (dict(page=48), 2), (dict(H=7), 2), (dict(n=0), 2), (dict(tokens=0), 2), (dict(pages=0), 2),
     (dict(bt_ld=2), 2), (dict(window=-1), 2), (dict(ldq=504), 2), (dict(stride=64), 7), (dict(stride=2 * 16 * 64 + 4), 7),
-    (dict(q=(1 << 20) + 2), 4), (dict(k=(1 << 21) + 8), 4), (dict(ldq=516), 4), (dict(sink=1 << 27, sink_dt=5), 3),
+    (dict(q=(1 << 20) + 2), 4), (dict(k=(1 << 21) + 8), 4), (dict(ldq=516), 4), (dict(sink=(1 << 27) + 4), 4),
     (dict(gate=1 << 27, ldg=7), 2), (dict(max_pages=1 << 28, bt_ld=1 << 28), 2)])
 def test_entry_points_refuse_before_the_device(kw, code):
     from zs_b200 import _lib, build
