@@ -1261,39 +1261,46 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
       if (loaded) ok = warp_wait(&q_full[t], q_n++ & 1, s_abort, ZS_DEVERR_TIMEOUT_EPILOGUE);
       if (!ok) break;
       if (a.k_sink != nullptr && loaded) {
-        // Head by head, a row's columns over the lanes, from the Q tile (swizzled 16-byte chunks); the
-        // next head's sink (from L2) is asked for ahead.  Little code and no division: what runs once a
-        // part is fetched anew each time.
-        const int col = lane * 4 & (HD - 1);
-        const uint8_t* qt = smem + L::OFF_Q + t * L::TILE + (col >> 6) * ATOM + (col & 4) * 2;
-        const float* sink = a.k_sink + (int64_t)b.hk * G * HD + col;
-        float4 w = __ldg(reinterpret_cast<const float4*>(sink));
+        // Q K_sink^T by mma.sync, 16 rows by 8 heads at a time, from which each row takes its own head's
+        // column; the f32 sink as the sum of two values of Q's type (2^-17 of it is lost).  Little code:
+        // what runs once a part is fetched anew each time, a few cycles an instruction.
         ok = warp_wait(&z_free[t], (z_n++ & 1) ^ 1, s_abort, ZS_DEVERR_TIMEOUT_EPILOGUE);
         if (!ok) break;
+        const uint32_t qt = smem_u32(smem + L::OFF_Q + t * L::TILE);
+        const int r4 = lane >> 2, c4 = lane & 3, inv = 65536 / G + 1;   // r / G == r * inv >> 16 for r < 128
 #pragma unroll 1
-        for (int g = 0; g < G; ++g) {
-          const float4 ahead = __ldg(reinterpret_cast<const float4*>(sink + (int64_t)min(g + 1, G - 1) * HD));
-#pragma unroll 1
-          for (int tr = 0; tr < tokens; tr += 8) {
-            float v[8];
+        for (int g0 = 0; g0 < G; g0 += 8) {
+          uint32_t hi[HD / 16][2], lo[HD / 16][2];
+          const float* sink = a.k_sink + (int64_t)(b.hk * G + min(g0 + r4, G - 1)) * HD + c4 * 2;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int row = min(tr + i, tokens - 1) * G + g;
-              float f[4];
-              unpack4<T>(*reinterpret_cast<const uint2*>(qt + row * 128 + (((col >> 3 & 7) ^ (row & 7)) << 4)), f);
-              v[i] = f[0] * w.x + f[1] * w.y + f[2] * w.z + f[3] * w.w;
+          for (int kk = 0; kk < HD / 16; ++kk)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const float2 f = __ldg(reinterpret_cast<const float2*>(sink + kk * 16 + x * 8));
+              const typename Pair<T>::type h2 = Pair<T>::from_f(f.x, f.y);
+              const float2 g2 = Pair<T>::to_f(h2);
+              const typename Pair<T>::type l2 = Pair<T>::from_f(f.x - g2.x, f.y - g2.y);
+              hi[kk][x] = *reinterpret_cast<const uint32_t*>(&h2);
+              lo[kk][x] = *reinterpret_cast<const uint32_t*>(&l2);
+            }
+#pragma unroll 1
+          for (int r0 = 0; r0 < G * tokens; r0 += 16) {
+            float acc[4] = {0.f, 0.f, 0.f, 0.f};
+            const int row = r0 + (lane & 15);
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; ++kk) {
+              const int ch = kk * 2 + (lane >> 4);
+              uint32_t q4[4];
+              ldsm_x4(qt + (ch >> 3) * ATOM + row * 128 + (((ch & 7) ^ (row & 7)) << 4), q4);
+              mma_16816<T>(acc, q4, hi[kk][0], hi[kk][1]);
+              mma_16816<T>(acc, q4, lo[kk][0], lo[kk][1]);
             }
 #pragma unroll
-            for (int off = HD / 8; off > 0; off >>= 1)
-#pragma unroll
-              for (int i = 0; i < 8; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], off);
-            if (lane == 0) {
-#pragma unroll
-              for (int i = 0; i < 8; ++i)
-                if (tr + i < tokens) s_z[t * PT_ROWS + (tr + i) * G + g] = v[i];
+            for (int x = 0; x < 2; ++x) {
+              const int r = r0 + r4 + x * 8, g = r - (r * inv >> 16) * G - g0;
+              if (g >> 1 == c4) s_z[t * PT_ROWS + r] = g & 1 ? acc[x * 2 + 1] : acc[x * 2];
             }
           }
-          w = ahead;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&z_full[t]);
