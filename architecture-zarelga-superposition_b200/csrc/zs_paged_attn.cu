@@ -8,6 +8,7 @@
 // logit or -inf.
 #include "zs_common.cuh"
 
+#include <atomic>
 #include <type_traits>
 
 namespace zs {
@@ -1632,6 +1633,18 @@ static int make_page_tmap(CUtensorMap* m, const void* base, int dtype, int hd, i
   return make_tmap3(m, base, dtype, hd, rows, pages, hd, page_stride, box_rows, 1);
 }
 
+// Shared memory beyond the default for a kernel, asked for once per device.
+template <auto KERNEL>
+static int allow_smem(int bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  ZS_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 64 && (done.load(std::memory_order_acquire) >> dev & 1)) return ZS_OK;
+  ZS_CUDA_TRY(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
+  return ZS_OK;
+}
+
 template <typename T, int HD>
 static int launch_decode(const paged::AttnArgs& a, int dtype, void* workspace, cudaStream_t stream) {
   using L = paged::DecSmem<HD>;
@@ -1649,7 +1662,8 @@ static int launch_decode(const paged::AttnArgs& a, int dtype, void* workspace, c
   const int resident = 2 * num_sms() < paged::DEC_MAX_BLOCKS ? 2 * num_sms() : paged::DEC_MAX_BLOCKS;
   const int blocks = (int)(all < resident ? all : resident);
   float* parts = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(workspace) + 15) & ~uintptr_t(15));
-  ZS_CUDA_TRY(cudaFuncSetAttribute(paged::paged_decode_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::ALLOC));
+  rc = allow_smem<paged::paged_decode_kernel<T, HD>>(L::ALLOC);
+  if (rc != ZS_OK) return rc;
   paged::paged_decode_kernel<T, HD><<<blocks, 160, L::ALLOC, stream>>>(tk, tv, a, parts);
   ZS_CUDA_TRY(cudaGetLastError());
   if (most == 1) return ZS_OK;                         // nothing can be split
@@ -1717,7 +1731,8 @@ static int launch_prompt(const paged::AttnArgs& a, int dtype, void* workspace, c
   const int grid = prompt_ctas(a.tokens, a.num_seqs, a.H, a.Hkv, a.max_pages, a.page, a.window);
   float* parts = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t(255));
   paged::PromptCut* cuts = reinterpret_cast<paged::PromptCut*>(parts + grid * 2 * paged::prompt_part_floats(HD));
-  ZS_CUDA_TRY(cudaFuncSetAttribute(paged::paged_prompt_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::ALLOC));
+  rc = allow_smem<paged::paged_prompt_kernel<T, HD>>(L::ALLOC);
+  if (rc != ZS_OK) return rc;
   paged::paged_prompt_kernel<T, HD><<<grid, paged::PT_THREADS, L::ALLOC, stream>>>(tq, tk, tv, a, parts, cuts);
   ZS_CUDA_TRY(cudaGetLastError());
   if (grid > 1 && (int64_t)a.max_pages * a.page > paged::PT_KEYS)      // else no block has a second tile to cut at

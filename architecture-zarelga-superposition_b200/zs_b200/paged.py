@@ -23,6 +23,7 @@ beyond the table, is skipped and recorded in the device error word (ZS_DEVERR_IN
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -150,7 +151,7 @@ def paged_append(qkvg, k_pages, v_pages, block_table, seq_lens, *, n_heads, cu_s
             cos, sin = cos.contiguous(), sin.contiguous()
             st = (rot, 1)
         table_ld = st[0]
-    q = torch.empty((T, H, hd), dtype=dtype, device=qkvg.device)
+    q = qkvg.new_empty((T, H, hd))
     if T == 0 or n == 0:
         return q.zero_()
     ld, inner = qkvg.stride()
@@ -167,6 +168,16 @@ def paged_append(qkvg, k_pages, v_pages, block_table, seq_lens, *, n_heads, cu_s
     if rc:
         Z.check(rc, "zs_paged_append")
     return q
+
+
+@functools.lru_cache(maxsize=64)
+def _decode_workspace(H, Hkv, hd):
+    return Z.lib().zs_paged_decode_workspace(1, H, Hkv, hd)   # the same for any number of sequences
+
+
+@functools.lru_cache(maxsize=256)
+def _prompt_workspace(*sizes):
+    return Z.lib().zs_paged_prompt_workspace(*sizes)
 
 
 def _attention(q, k_pages, v_pages, block_table, seq_lens, cu_seqlens, window, k_sink, gate, scale, return_lse, decode):
@@ -202,7 +213,7 @@ def _attention(q, k_pages, v_pages, block_table, seq_lens, cu_seqlens, window, k
             gate = gate.contiguous()
             ldg = H
         ldg = max(ldg, H)
-    o = torch.empty((T, H, hd), dtype=dtype, device=q.device)
+    o = q.new_empty((T, H, hd))
     lse = torch.empty((T, H), dtype=torch.float32, device=q.device) if return_lse else None
     if T == 0 or n == 0:
         o.zero_()
@@ -221,11 +232,11 @@ def _attention(q, k_pages, v_pages, block_table, seq_lens, cu_seqlens, window, k
     stream = torch._C._cuda_getCurrentRawStream(dev)
     Z.count(2)
     if decode:
-        size = L.zs_paged_decode_workspace(n, H, Hkv, hd)
+        size = _decode_workspace(H, Hkv, hd)
         ws = torch.empty(size, dtype=torch.uint8, device=q.device)
         rc = L.zs_paged_decode_attention(*args, n, *more, ws.data_ptr(), size, stream)
     else:
-        size = L.zs_paged_prompt_workspace(T, n, H, Hkv, hd, m, page, w)
+        size = _prompt_workspace(T, n, H, Hkv, hd, m, page, w)
         ws = torch.empty(size, dtype=torch.uint8, device=q.device)
         rc = L.zs_paged_prompt_attention(*args, cu_seqlens.data_ptr(), n, T, *more, ws.data_ptr(), size, stream)
     if rc:
