@@ -10,6 +10,9 @@
 namespace zs {
 namespace paged {
 
+// Tokens of a sequence: positions rounded up to a tile stay below 2^31.
+constexpr int64_t MAX_TOKENS = ((int64_t)1 << 31) - 256;
+
 // ------------------------------------------------------------------ element helpers
 
 template <typename T>
@@ -624,7 +627,7 @@ static int cache_ok(const zs_kv_cache* c) {
                  c->max_seqs >= 1 && c->max_pages >= 1,
              ZS_ERR_SHAPE);
   ZS_REQUIRE(c->page_size == 16 || c->page_size == 32 || c->page_size == 64 || c->page_size == 128, ZS_ERR_SHAPE);
-  ZS_REQUIRE((int64_t)c->max_pages * c->page_size < (int64_t)1 << 31, ZS_ERR_SHAPE);
+  ZS_REQUIRE((int64_t)c->max_pages * c->page_size <= MAX_TOKENS, ZS_ERR_SHAPE);
   ZS_REQUIRE(c->head_dim == 64 || c->head_dim == 128, ZS_ERR_SHAPE);
   ZS_REQUIRE((reinterpret_cast<uintptr_t>(c->kv) & 15) == 0, ZS_ERR_ALIGN);
   return ZS_OK;
@@ -761,7 +764,7 @@ static int pages_ok(const void* k_pages, const void* v_pages, int64_t page_strid
   ZS_REQUIRE(page == 16 || page == 32 || page == 64 || page == 128, ZS_ERR_SHAPE);
   ZS_REQUIRE(H >= 1 && Hkv >= 1 && H % Hkv == 0 && H <= 65535, ZS_ERR_SHAPE);
   ZS_REQUIRE(num_seqs >= 1 && tokens >= 1 && tokens < (int64_t)1 << 31 && num_pages >= 1 &&
-                 num_pages < (int64_t)1 << 30 && max_pages >= 1 && (int64_t)max_pages * page < (int64_t)1 << 31,
+                 num_pages < (int64_t)1 << 30 && max_pages >= 1 && (int64_t)max_pages * page <= paged::MAX_TOKENS,
              ZS_ERR_SHAPE);
   ZS_REQUIRE(bt_ld >= max_pages, ZS_ERR_SHAPE);
   ZS_REQUIRE(page_stride >= (int64_t)Hkv * page * hd && page_stride % 8 == 0, ZS_ERR_LAYOUT);

@@ -602,10 +602,12 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const AttnA
   const Runs runs(total * units, decode_blocks);
   const int64_t t0 = before * units + (int64_t)unit * steps + OVER, t1 = t0 + steps - OVER - 1;   // its first and last tile
   const int b0 = (int)runs.block_of(t0), b1 = (int)runs.block_of(t1);
+  // every block waits, also one with nothing to join: what follows this grid in the stream follows the
+  // decode kernel only through it
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (b0 == b1) return;
   // a block's first part lies in its slot 0; the first block's part may come after another one
   const int shift = runs.begin(b0) < t0 - OVER ? 1 : 0;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int shares = nrow >= JOIN_WARPS ? 1 : JOIN_WARPS / nrow;
   const int share = warp % shares, sub = lane / (HD / 4), col = (lane % (HD / 4)) * 4;
   for (int row = warp / shares; row < nrow; row += JOIN_WARPS / shares) {
@@ -1576,6 +1578,7 @@ static int attn_args(paged::AttnArgs& a, const void* q, int64_t ldq, const void*
                           tokens, H, Hkv, hd, page, dtype);
   if (rc != ZS_OK) return rc;
   ZS_REQUIRE(q && o, ZS_ERR_ARG);
+  ZS_REQUIRE(scale >= 0.f, ZS_ERR_ARG);                // the running maximum is of S, then scaled
   ZS_REQUIRE(window >= 0 && ldq >= (int64_t)H * hd && (gate == nullptr || ldg >= H), ZS_ERR_SHAPE);
   ZS_REQUIRE(ldq % 8 == 0 && ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(o)) & 15) == 0, ZS_ERR_ALIGN);
   ZS_REQUIRE((reinterpret_cast<uintptr_t>(k_sink) & 15) == 0, ZS_ERR_ALIGN);

@@ -64,7 +64,7 @@ def sample(logits, temperature=0.0, generator=None):
 def generate(model, prompts, max_new_tokens, *, temperature=0.0, eos_token_id=None, page_size=64, generator=None):
     """Continuations (a list of lists of ids) of prompts (a list of non-empty id sequences).  Greedy
     by default; a sequence ends after eos_token_id (which is part of it) or max_new_tokens ids."""
-    prompts = [torch.as_tensor(p, dtype=torch.long) for p in prompts]
+    prompts = [torch.as_tensor(p, dtype=torch.long).reshape(-1) for p in prompts]
     if not prompts or min(p.numel() for p in prompts) < 1:
         raise Z.ZsError("generate needs prompts of at least one token")
     if max_new_tokens < 1:

@@ -223,7 +223,10 @@ def _attention(q, k_pages, v_pages, block_table, seq_lens, cu_seqlens, window, k
     if inner != 1 or (head != hd and H > 1) or ldq % 8 or x % 16 or (T > 1 and ldq < H * hd):
         q = q.clone(memory_format=torch.contiguous_format)
         x, ldq = q.data_ptr(), H * hd
-    scale = 1.0 / math.sqrt(hd) if scale is None else scale
+    if scale is None:
+        scale = 1.0 / math.sqrt(hd)
+    elif not scale >= 0.0:
+        _fail(f"scale must not be negative (got {scale!r})")
     L = Z.lib()
     args = (x, max(ldq, H * hd), k_pages.data_ptr(), v_pages.data_ptr(), stride, P, block_table.data_ptr(), bt_ld, m,
             seq_lens.data_ptr())
@@ -285,7 +288,7 @@ class PagedKVCache:
             _fail(f"the cache holds bf16 or f16 pages of {PAGE_SIZES} tokens of head_dim 64 or 128 (got {dtype}, "
                   f"{page_size}, {head_dim})")
         if (min(n_layers, n_kv_heads, num_pages, max_seqs, max_pages_per_seq) < 1 or num_pages > 2_000_000
-                or max_pages_per_seq * page_size >= 1 << 31):
+                or max_pages_per_seq * page_size > (1 << 31) - 256):
             _fail("n_layers, n_kv_heads, num_pages (at most 2000000), max_seqs and max_pages_per_seq must be positive")
         self.kv = torch.zeros(n_layers, 2, num_pages, n_kv_heads, page_size, head_dim, dtype=dtype, device=device)
         cells = max_seqs * max_pages_per_seq

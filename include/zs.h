@@ -691,7 +691,7 @@ int zs_sparse_rmsprop_step(float* param, int64_t num_rows, int64_t d, int64_t ld
  *   key: o is zero (lse of padding outside every sequence: -inf).  A NaN or
  *   infinity in a value of the sequence may reach every row of the same
  *   sequence; what lies in the pages outside the sequence reaches none.
- *   H / Hkv <= 128.
+ *   H / Hkv <= 128; scale >= 0.
  *   Both attentions split long work over thread blocks and join the parts in a
  *   fixed order; the workspace holds the parts of this call only, so calls that
  *   may overlap need one each.

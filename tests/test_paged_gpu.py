@@ -165,6 +165,34 @@ def test_prompt_few_sequences(lens, new, hd):
     _check(w, o, lse)
 
 
+@pytest.mark.parametrize("H,Hkv,hd", [(128, 1, 64), (100, 1, 128), (66, 2, 64), (17, 1, 128)])
+def test_large_groups(H, Hkv, hd):
+    """Few tokens a tile, several blocks of query heads in a decode step, sinks in many columns."""
+    from zs_b200 import paged
+
+    lens, new = [1, 40, 300], [1, 7, 9]
+    w = _world(lens, new, H=H, Hkv=Hkv, hd=hd, page=16, dtype=torch.bfloat16, sink=torch.float32, gate=True, seed=H)
+    o, lse = paged.paged_prompt_attention(w["q"], w["k"], w["v"], w["table"], w["lens"], w["cu"], k_sink=w["ks"],
+                                          gate=w["gate"], return_lse=True)
+    _check(w, o, lse)
+    w = _world(lens, [1] * 3, H=H, Hkv=Hkv, hd=hd, page=16, dtype=torch.bfloat16, sink=torch.float32, gate=True, seed=H)
+    o, lse = paged.paged_decode_attention(w["q"], w["k"], w["v"], w["table"], w["lens"], k_sink=w["ks"],
+                                          gate=w["gate"], return_lse=True)
+    _check(w, o, lse)
+
+
+@pytest.mark.parametrize("lens,new", [([5], [9]), ([0, 3], [30, 200]), ([130], [400])])
+def test_prompt_before_the_first_position(lens, new):
+    """Tokens at negative positions (more new tokens than the sequence is long): zero rows, whose
+    log-sum-exp is the sink's logit."""
+    from zs_b200 import paged
+
+    w = _world(lens, new, H=6, Hkv=2, hd=64, page=16, dtype=torch.float16, sink=torch.float32, gate=True)
+    o, lse = paged.paged_prompt_attention(w["q"], w["k"], w["v"], w["table"], w["lens"], w["cu"], k_sink=w["ks"],
+                                          gate=w["gate"], return_lse=True)
+    _check(w, o, lse)
+
+
 def test_prompt_rows_of_no_sequence_are_zero():
     from zs_b200 import paged
 
@@ -458,7 +486,7 @@ def test_refusals():
     bad = [dict(q=w["q"].half()), dict(q=w["q"][:, :3]), dict(q=w["q"].cpu()), dict(k=w["k"].float(), v=w["v"].float()),
            dict(k=w["k"][:, :, :8], v=w["v"][:, :, :8]), dict(k=w["k"].transpose(1, 2)), dict(v=w["v"][:, :1]),
            dict(table=w["table"].long()), dict(table=w["table"][0]), dict(lens=w["lens"].long()),
-           dict(lens=w["lens"][:1]), dict(cu=w["cu"][:2]), dict(cu=w["cu"].long()), dict(window=0), dict(window=-3),
+           dict(scale=-1.0), dict(scale=float("nan")), dict(lens=w["lens"][:1]), dict(cu=w["cu"][:2]), dict(cu=w["cu"].long()), dict(window=0), dict(window=-3),
            dict(k_sink=torch.zeros(3, 64, device="cuda")), dict(gate=torch.zeros(5, 4, device="cuda")),
            dict(gate=torch.zeros(4, 4, device="cuda", dtype=torch.bfloat16)),
            dict(q=w["q"].clone().requires_grad_(True)), dict(table=w["table"][:1].expand(2, -1))]
@@ -555,6 +583,65 @@ def test_bookkeeping_and_append_in_a_graph():
     for s in range(3):
         for p in range(1, 41):
             assert torch.equal(v[ref.table[s][p // 16], :, p % 16].flatten(), x[s, 256:])
+
+
+def test_prompt_and_page_moves_in_graphs():
+    """A prompt, a fork, a compaction and a copy recorded and replayed, two prompts at once."""
+    from zs_b200 import paged
+
+    ws = [_world([700, 90], [500, 90], H=8, Hkv=2, hd=128, page=32, dtype=torch.bfloat16, seed=s) for s in (3, 4)]
+
+    def call(w):
+        return paged.paged_prompt_attention(w["q"], w["k"], w["v"], w["table"], w["lens"], w["cu"])
+
+    want = [call(w) for w in ws]
+    graphs, outs = [], []
+    for w in ws:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(call(w))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in ws]
+    for _ in range(10):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for o, r in zip(outs, want):
+        assert torch.equal(o, r)
+
+    c, ref = _cache(P=40, page=16, slots=6, M=9)
+    c.extend([0, 1, 2, 3], [40, 33, 48, 100]), ref.extend([0, 1, 2, 3], [40, 33, 48, 100])
+    i32 = dict(dtype=torch.int32, device="cuda")
+    src, dst, one = (torch.tensor(x, **i32) for x in ([1, 0, 3], [0, 4, 5], [2, 1]))
+    a, b = torch.tensor([0, 3], **i32), torch.tensor([39, 38], **i32)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        c.fork(src, dst)
+        c.free(one)
+        c.compact()
+        c.copy_pages(a, b)
+    for _ in range(3):
+        g.replay()
+        ref.fork([1, 0, 3], [0, 4, 5]), ref.free([2, 1]), ref.compact(), ref.copy_pages([0, 3], [39, 38])
+        c.extend([1, 2], [20, 5]), ref.extend([1, 2], [20, 5])
+    _same(c, ref)
+
+
+def test_work_behind_a_call_sees_its_results():
+    """Nothing to join (one tile a sequence): what follows in the stream still waits for the call."""
+    from zs_b200 import paged
+
+    w = _world([60] * 600, [1] * 600, H=16, Hkv=16, hd=128, page=64, dtype=torch.bfloat16, poison=False)
+    table = w["table"].contiguous()
+    want = paged.paged_decode_attention(w["q"], w["k"], w["v"], table, w["lens"]).clone()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = paged.paged_decode_attention(w["q"], w["k"], w["v"], table, w["lens"])
+        copy = got.clone()
+        got.zero_()
+        assert torch.equal(copy, want)
+        assert (got == 0).all()
 
 
 def test_another_stream():

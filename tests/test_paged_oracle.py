@@ -51,7 +51,7 @@ def _attn_args(**kw):
 @pytest.mark.parametrize("kw,code", [
     (dict(q=None), 1), (dict(o=None), 1), (dict(table=None), 1), (dict(cu=None), 1), (dict(dtype=0), 3),
     (dict(hd=96), 2), (dict(page=48), 2), (dict(H=7), 2), (dict(n=0), 2), (dict(tokens=0), 2), (dict(pages=0), 2),
-    (dict(bt_ld=2), 2), (dict(window=-1), 2), (dict(ldq=504), 2), (dict(stride=64), 7), (dict(stride=2 * 16 * 64 + 4), 7),
+    (dict(bt_ld=2), 2), (dict(window=-1), 2), (dict(scale=-0.1), 1), (dict(ldq=504), 2), (dict(stride=64), 7), (dict(stride=2 * 16 * 64 + 4), 7),
     (dict(q=(1 << 20) + 2), 4), (dict(k=(1 << 21) + 8), 4), (dict(ldq=516), 4), (dict(sink=(1 << 27) + 4), 4),
     (dict(gate=1 << 27, ldg=7), 2), (dict(max_pages=1 << 28, bt_ld=1 << 28), 2)])
 def test_entry_points_refuse_before_the_device(kw, code):
@@ -64,7 +64,7 @@ def test_entry_points_refuse_before_the_device(kw, code):
     if "cu" not in kw and "tokens" not in kw:
         d = args[:10] + [args[11]] + args[13:]
         assert L.zs_paged_decode_attention(*d, 1 << 28, 1 << 40, None) == code
-    if not kw.keys() & {"o", "window", "sink", "gate", "ldq", "cu", "q"}:
+    if not kw.keys() & {"o", "window", "scale", "sink", "gate", "ldq", "cu", "q"}:
         a = dict(zip(("q", "ldq", "k", "v", "stride", "pages", "table", "bt_ld", "max_pages", "lens", "cu", "n",
                       "tokens", "H", "Hkv", "hd", "page"), args))
         assert L.zs_paged_append(a["q"], 2048, None, None, 1e-6, None, None, 0, 0, 0, a["k"], a["v"], a["stride"],
