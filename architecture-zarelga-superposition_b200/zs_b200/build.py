@@ -1,13 +1,16 @@
 """Build libzs.so (all sm_100a kernels + the C ABI) in-tree with nvcc.
 
 The library is a plain shared object: no torch headers, no Python API.  It is
-written next to this file so it travels with the source tree.
+written next to this file so it travels with the source tree.  Beside it
+_paged.so, a small host-only binding of the paged cache operators to CPython and
+torch, is compiled with g++ and linked against it.
 """
 from __future__ import annotations
 
 import os
 import shutil
 import subprocess
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -15,6 +18,7 @@ ROOT = PKG.parent
 CSRC = ROOT / "csrc"
 INCLUDE = ROOT.parent / "include"
 LIB = PKG / "libzs.so"
+BINDING = PKG / "_paged.so"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -42,15 +46,46 @@ def needs_build() -> bool:
     return any(p.stat().st_mtime > t for p in sources())
 
 
-def build(force: bool = False, verbose: bool = False) -> Path:
-    if not force and not needs_build():
-        return LIB
-    tmp = LIB.with_suffix(".so.tmp")
-    cmd = [_nvcc(), *NVCC_FLAGS, "-I", str(INCLUDE), "-o", str(tmp), str(CSRC / "zs_lib.cu")]
+def binding_needs_build() -> bool:
+    if not BINDING.exists():
+        return True
+    t = BINDING.stat().st_mtime
+    return any(p.stat().st_mtime > t for p in (CSRC / "zs_paged_py.cpp", INCLUDE / "zs.h"))
+
+
+def build_binding(force: bool = False, verbose: bool = False) -> Path:
+    if not force and not binding_needs_build():
+        return BINDING
+    import torch
+
+    cxx = shutil.which("g++")
+    if cxx is None:
+        raise RuntimeError("g++ not found: the paged operators' binding cannot be built")
+    t = Path(torch.__file__).resolve().parent
+    cuda = Path(_nvcc()).resolve().parent.parent
+    tmp = BINDING.with_suffix(".so.tmp")
+    cmd = [cxx, "-O2", "-std=c++17", "-shared", "-fPIC",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", str(INCLUDE),
+           "-I", sysconfig.get_paths()["include"], "-I", str(t / "include"),
+           "-I", str(t / "include" / "torch" / "csrc" / "api" / "include"), "-I", str(cuda / "include"),
+           "-o", str(tmp), str(CSRC / "zs_paged_py.cpp"), "-L", str(PKG), "-l:libzs.so", "-L", str(t / "lib"),
+           "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
     if verbose:
         print(" ".join(cmd))
     subprocess.run(cmd, check=True)
-    os.replace(tmp, LIB)
+    os.replace(tmp, BINDING)
+    return BINDING
+
+
+def build(force: bool = False, verbose: bool = False) -> Path:
+    if force or needs_build():
+        tmp = LIB.with_suffix(".so.tmp")
+        cmd = [_nvcc(), *NVCC_FLAGS, "-I", str(INCLUDE), "-o", str(tmp), str(CSRC / "zs_lib.cu")]
+        if verbose:
+            print(" ".join(cmd))
+        subprocess.run(cmd, check=True)
+        os.replace(tmp, LIB)
+    build_binding(force, verbose)
     return LIB
 
 
