@@ -31,16 +31,6 @@ struct Pair<__half> {
 };
 
 template <typename T>
-__device__ __forceinline__ void unpack8(const uint4& u, float (&v)[8]) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = Pair<T>::to_f(*reinterpret_cast<const typename Pair<T>::type*>(&w[i]));
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
-  }
-}
-template <typename T>
 __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
   uint32_t w[4];
 #pragma unroll

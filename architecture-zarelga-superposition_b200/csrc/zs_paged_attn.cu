@@ -30,7 +30,7 @@ struct AttnArgs {
   int64_t tokens;
   int H, Hkv, page;
   int window;                  // 0: none
-  float scale, scale_log2;
+  float scale_log2;            // softmax scale * log2(e)
   const float* k_sink;         // nullable [H, hd]
   const void* gate;            // nullable [tokens, H] rows of ldg elements
   int64_t ldg;
@@ -61,6 +61,9 @@ __device__ __forceinline__ int cut_length(const AttnArgs& a, int seq) {
 // as the 16 rows, P straight from the accumulators of S, and a running (max, sum, O) of their
 // own, joined through shared memory when a part ends.  mma.sync, not tcgen05: a 128-row tile
 // would hold 1 to 16 rows of work, and the products are a tenth of the time of the loads.
+//
+// 64 sequences of 30K to 32K tokens, 16/4 heads of 128: 610 us, 6.7 TB/s (a copy reaches 6.56); 32 of 1 to
+// 4096 tokens, 12/4 heads: 30 us, of which 20 are the bytes, 3.4 the start to the first load.
 
 constexpr int DEC_MAX_BLOCKS = 320;       // two per SM
 constexpr int DEC_ROWS = 16;              // query heads per block of rows
@@ -692,10 +695,16 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const AttnA
 //   warp 0      TMA: both Q tiles, then K and V of 128 keys, page by page, into a ring of slots
 //   warp 1      MMA: per key tile and query tile t, O_t += P_t V (P from tensor memory, the first
 //               half of its keys as soon as that half is there), then S_t = Q_t K^T
+//   warps 2, 3  rows of no sequence (zero); the sink logits of query tiles 0 and 1
 //   warps 4..7  softmax of query tile 0, warps 8..11 of query tile 1: one row per thread; S from
 //               tensor memory, running max (log2 units, raised when it grows by more than 2^8)
 //               and sum, P in the cache's type over S's first 64 columns, at the end the row out
-// TMEM columns: S_t / P_t at t * 128, O_t at 256 + t * hd.
+// TMEM columns: S_t / P_t at t * 128, O_t at 256 + t * hd.  P is rounded to the cache's type because the
+// products take 16-bit operands; its sum is taken in f32 before that.
+//
+// One prompt of 32768 tokens, 16/4 heads of 128: 4.05 ms, 1086 TFLOP/s (64 % of a cuBLAS burst).  Bound by
+// the chain of a query tile: of 3850 cycles for a step of both tiles, softmax takes 2000, products and
+// waits 1700 to 1800, and the two tiles overlap each other's; pure products would take 2100.
 
 constexpr int PT_ROWS = 128;              // rows of a query tile
 constexpr int PT_KEYS = 128;              // keys of a key tile
@@ -1599,7 +1608,6 @@ static int attn_args(paged::AttnArgs& a, const void* q, int64_t ldq, const void*
   a.Hkv = Hkv;
   a.page = page;
   a.window = window;
-  a.scale = scale;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.k_sink = k_sink;
   a.gate = gate;
