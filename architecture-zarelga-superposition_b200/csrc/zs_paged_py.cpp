@@ -5,6 +5,7 @@
 // around ctypes took 17 us a call besides the launches, these take about 2, so this is the one part of the
 // package that is bound through CPython and torch's C++ API; the kernels stay in libzs.so behind include/zs.h.
 #include <Python.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/torch.h>
@@ -159,12 +160,13 @@ PyObject* append(PyObject* const* a) {
   const at::Tensor *wq = maybe(a[7], "q_weight"), *wk = maybe(a[8], "k_weight");
   const double eps = real(a[9], "eps");
   const at::Tensor *cos = maybe(a[10], "cos"), *sin = maybe(a[11], "sin");
-  Inputs in(k);
+  const Inputs in(k);
+  const c10::cuda::CUDAGuard on(in.device);   // the library makes that device current
   for (const at::Tensor* t : {&v, (const at::Tensor*)&x, &table, &lens, cu, wq, wk, cos, sin}) in.add(t);
   const Pages p(k, v);
   const Tables tab(table, lens, cu);
   const int64_t width = (H + 2 * p.heads) * p.hd;
-  if (x.dim() != 2 || x.scalar_type() != p.dtype || H < 1 || H % p.heads || x.size(1) < width)
+  if (x.dim() != 2 || x.scalar_type() != p.dtype || H < 1 || H > x.size(1) || H % p.heads || x.size(1) < width)
     refuse("qkvg must be ", p.dtype, " [T, >= (H + 2 Hkv) hd] with H % Hkv == 0 (got ", x.scalar_type(), " ", x.sizes(),
            ", H=", H, ", Hkv=", p.heads, ", hd=", p.hd, ")");
   const int64_t T = x.size(0);
@@ -223,7 +225,8 @@ PyObject* attention(PyObject* const* a) {
   const at::Tensor* cu = maybe(a[5], "cu_seqlens");
   const bool decode = cu == nullptr;
   const at::Tensor *sink_in = maybe(a[7], "k_sink"), *gate_in = maybe(a[8], "gate");
-  Inputs in(k);
+  const Inputs in(k);
+  const c10::cuda::CUDAGuard on(in.device);   // the library makes that device current
   for (const at::Tensor* t : {&v, (const at::Tensor*)&q, &table, &lens, cu, sink_in, gate_in}) in.add(t);
   const Pages p(k, v);
   const Tables tab(table, lens, cu);
@@ -320,6 +323,7 @@ PyObject* pages(PyObject* const* a) {
   }
   if (lists[0] && lists[1] && lists[0]->size(0) != lists[1]->size(0)) refuse("request lists must have one length");
   if (op != 3 && n == 0) Py_RETURN_NONE;
+  const c10::cuda::CUDAGuard on(kv.device());
   void* stream = c10::cuda::getCurrentCUDAStream(kv.get_device()).stream();
   const int* x = static_cast<const int*>(ptr(lists[0]));
   const int* y = static_cast<const int*>(ptr(lists[1]));

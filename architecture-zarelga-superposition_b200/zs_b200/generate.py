@@ -16,7 +16,11 @@ from .dense import one_group_routing
 class DecodeStep:
     """One decode step of all slots of a cache as a CUDA graph: the slots grow by `active` (0 or 1)
     tokens, `tokens` go in, `logits` come out.  An inactive slot's row is computed and ignored; its
-    newest token's keys are overwritten, so it must not be continued later."""
+    newest token's keys are overwritten, so it must not be continued later.
+
+    The recorded kernels read the weights' bf16 shadows where they lay at the recording.  The
+    package's optimizer writes those with the weights; after any other change of a weight (a
+    torch operation, load_state_dict, another parameter in its place) the step is recorded again."""
 
     def __init__(self, model, cache):
         dev = cache.kv.device
@@ -33,21 +37,33 @@ class DecodeStep:
         c.extend(self.slots, self.active)
         return self.model.forward_paged(self.tokens, c, c.block_table, c.seq_lens)
 
+    @staticmethod
+    def _place(p):
+        """Where a kernel reads parameter p, and the change by torch that its shadow is in step with."""
+        sh = getattr(p, "_zs_sh", None)
+        return p.data_ptr(), None if sh is None else (sh.data_ptr(), p._version)
+
+    def _current(self):
+        return all(held.get(name) is p and self._place(p) == place for held, name, p, place in self._read)
+
     def __call__(self):
-        if self.graph is None:
-            # the first step warms up every lazily made buffer outside the recording (it is a real
-            # step), then the next ones are recorded
-            self.logits = self._run()
-            # tensors that other code may drop while the graph still reads them
-            self._held = one_group_routing(self.tokens.numel(), self.tokens.device)
-            torch.cuda.current_stream(self.tokens.device).synchronize()
+        if self.graph is not None and self._current():
+            self.graph.replay()
+            self.logits = self._static
+            return self.logits
+        # a step outside the recording first (a real one): it makes or refreshes every lazily
+        # made buffer, then the next ones are recorded
+        self.logits = self._run()
+        # tensors that other code may drop while the graph still reads them
+        self._held = one_group_routing(self.tokens.numel(), self.tokens.device)
+        with torch.cuda.device(self.tokens.device):
+            torch.cuda.current_stream().synchronize()
             graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(graph):
                 self._static = self._run()
-            self.graph = graph
-            return self.logits
-        self.graph.replay()
-        self.logits = self._static
+        self._read = [(m._parameters, name, p, self._place(p)) for m in self.model.modules()
+                      for name, p in m._parameters.items() if p is not None]
+        self.graph = graph
         return self.logits
 
 

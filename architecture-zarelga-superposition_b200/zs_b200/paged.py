@@ -114,7 +114,8 @@ class PagedKVCache:
                   f"{page_size}, {head_dim})")
         if (min(n_layers, n_kv_heads, num_pages, max_seqs, max_pages_per_seq) < 1 or num_pages > 2_000_000
                 or max_pages_per_seq * page_size > (1 << 31) - 256):
-            _fail("n_layers, n_kv_heads, num_pages (at most 2000000), max_seqs and max_pages_per_seq must be positive")
+            _fail("n_layers, n_kv_heads, num_pages (at most 2000000), max_seqs and max_pages_per_seq (at most "
+                  "2^31 - 256 tokens) must be positive")
         self.kv = torch.zeros(n_layers, 2, num_pages, n_kv_heads, page_size, head_dim, dtype=dtype, device=device)
         cells = max_seqs * max_pages_per_seq
         self.meta = torch.empty(cells + max_seqs + num_pages, dtype=torch.int32, device=device)

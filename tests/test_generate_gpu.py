@@ -116,6 +116,43 @@ def test_generate_is_greedy_and_stops():
     assert len(hot[0]) == 8 and all(0 <= t < cfg.vocab_size for t in hot[0])
 
 
+@pytest.mark.parametrize("change", ["in_place", "load", "replaced", "moved"])
+def test_a_recorded_step_follows_its_weights(change):
+    from zs_b200.generate import DecodeStep
+
+    cfg, m = _model()
+    c = m.new_cache(2, 64, page_size=16)
+    step = DecodeStep(m, c)
+    step.active.fill_(1)
+    step.tokens.copy_(torch.tensor([3, 9]))
+    for _ in range(3):
+        step()
+    recorded = step.graph
+    step()
+    assert step.graph is recorded
+    with torch.no_grad():
+        if change == "in_place":
+            m.layers[1].self_attn.o_proj.weight.mul_(-1.5)
+        elif change == "load":
+            m.load_state_dict({k: v * 1.25 if k.endswith("q_proj.weight") else v for k, v in m.state_dict().items()})
+        elif change == "replaced":
+            w = m.layers[0].self_attn.v_proj.weight
+            m.layers[0].self_attn.v_proj.weight = torch.nn.Parameter(w * -2)
+        else:
+            w = m.output_layer.weight
+            w.data = w.data * 3
+    snapshot, kv = c.meta.clone(), c.kv.clone()
+    for _ in range(3):                       # recorded anew, then replayed
+        got = step().clone()
+        c.meta.copy_(snapshot)
+        c.kv.copy_(kv)
+        c.extend(step.slots, step.active)
+        want = m.forward_paged(step.tokens, c, c.block_table, c.seq_lens)
+        assert torch.equal(got, want)
+        snapshot, kv = c.meta.clone(), c.kv.clone()
+    c.check()
+
+
 def test_generate_refuses():
     from zs_b200 import ZsError
 
