@@ -310,10 +310,24 @@ __device__ __forceinline__ void hold(const zs_kv_cache& c, int page, int by) {
     record_error(ZS_DEVERR_INDEX);
 }
 
+// Up to PLAN_THREADS requests keep their part of the plan in shared memory: what the block
+// writes and reads again would otherwise be a trip to L2 each time.  The counts, which it
+// searches in the end, are asked for at its start.
+struct PlanShared {
+  int warp[32], first[PLAN_SLOTS], off[PLAN_THREADS], len[PLAN_THREADS], free_pages[PLAN_THREADS];
+};
+__device__ __forceinline__ Plan in_shared(const zs_kv_cache& c, Plan p, int n, PlanShared& s) {
+  if (c.max_seqs <= PLAN_SLOTS) p.first = s.first;
+  if (n <= PLAN_THREADS) p.off = s.off, p.len = s.len;
+  if ((int64_t)threadIdx.x * 32 < c.num_pages)
+    asm volatile("prefetch.global.L1 [%0];" ::"l"(c.ref_count + threadIdx.x * 32));
+  return p;
+}
+
 // Each request's number of new pages (need_of(i), -1: refused) scanned in
 // order into plan.off; the pages found; requests past them refused.
 template <typename F>
-__device__ __forceinline__ void allot(const zs_kv_cache& c, const Plan& p, int n, F need_of, int* s_warp) {
+__device__ __forceinline__ void allot(const zs_kv_cache& c, Plan& p, int n, F need_of, int* s_warp, int* s_free) {
   int total = 0;
   for (int i0 = 0; i0 < n; i0 += PLAN_THREADS) {
     const int i = i0 + threadIdx.x;
@@ -327,6 +341,7 @@ __device__ __forceinline__ void allot(const zs_kv_cache& c, const Plan& p, int n
   }
   __syncthreads();
   const int want = total > (int)c.num_pages ? (int)c.num_pages : total;
+  if (want <= PLAN_THREADS) p.free_pages = s_free;
   const int have = find_free(c.ref_count, c.num_pages, want, p.free_pages, s_warp);
   for (int i = threadIdx.x; i < n; i += PLAN_THREADS) {
     const int need = need_of(i);
@@ -338,40 +353,54 @@ __device__ __forceinline__ void allot(const zs_kv_cache& c, const Plan& p, int n
   __syncthreads();
 }
 
-__global__ void __launch_bounds__(PLAN_THREADS) kv_extend_kernel(const zs_kv_cache c, Plan p, const int* slots,
-                                                                 const int* tokens, int n) {
-  __shared__ int s_warp[32], s_first[PLAN_SLOTS];
-  if (c.max_seqs <= PLAN_SLOTS) p.first = s_first;
+__global__ void __launch_bounds__(PLAN_THREADS) kv_extend_kernel(const zs_kv_cache c, const Plan plan,
+                                                                 const int* slots, const int* tokens, int n) {
+  __shared__ PlanShared sh;
+  Plan p = in_shared(c, plan, n, sh);
   mark_first(slots, n, c.max_seqs, p.first);
   auto need_of = [&](int i) -> int {
     const int s = slots[i], t = tokens[i];
     if ((unsigned)s >= (unsigned)c.max_seqs || t < 0 || p.first[s] != i) return -1;
     const int len = c.seq_lens[s];
     const int64_t end = (int64_t)len + t;
-    if (end > (int64_t)c.max_pages * c.page_size) return -1;
+    if (len < 0 || end > (int64_t)c.max_pages * c.page_size) return -1;
     return (int)((end + c.page_size - 1) / c.page_size) - (len + c.page_size - 1) / c.page_size;
   };
   for (int i = threadIdx.x; i < n; i += PLAN_THREADS) {
     const int s = slots[i], t = tokens[i];
-    if ((unsigned)s >= (unsigned)c.max_seqs || t < 0 || p.first[s] != i)
+    if ((unsigned)s >= (unsigned)c.max_seqs || t < 0 || p.first[s] != i || c.seq_lens[s] < 0)
       record_error(ZS_DEVERR_INDEX);
     else if ((int64_t)c.seq_lens[s] + t > (int64_t)c.max_pages * c.page_size)
       record_error(ZS_DEVERR_CACHE_FULL);
   }
-  allot(c, p, n, need_of, s_warp);
-  const int lane = threadIdx.x & 31;
-  for (int i = threadIdx.x >> 5; i < n; i += PLAN_THREADS / 32) {   // a warp per request
+  allot(c, p, n, need_of, sh.warp, sh.free_pages);
+  // A thread writes a request's first pages, a warp the many of a prompt.
+  constexpr int FEW = 2;
+  for (int i = threadIdx.x; i < n; i += PLAN_THREADS) {
     const int off = p.off[i];
     if (off < 0) continue;
-    const int s = slots[i], need = need_of(i), len = c.seq_lens[s];
+    const int s = slots[i], len = c.seq_lens[s], need = need_of(i);
     const int old = (len + c.page_size - 1) / c.page_size;
-    __syncwarp();
-    for (int j = lane; j < need; j += 32) {
+    for (int j = 0; j < min(need, FEW); ++j) {
       const int pg = p.free_pages[off + j];
       c.block_table[(int64_t)s * c.max_pages + old + j] = pg;
       c.ref_count[pg] = 1;
     }
-    if (lane == 0) c.seq_lens[s] = len + tokens[i];
+    p.len[i] = need;
+    p.rows[i] = old;
+    c.seq_lens[s] = len + tokens[i];
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & 31;
+  for (int i = threadIdx.x >> 5; i < n; i += PLAN_THREADS / 32) {
+    const int off = p.off[i];
+    if (off < 0 || p.len[i] <= FEW) continue;
+    int* row = c.block_table + (int64_t)slots[i] * c.max_pages + p.rows[i];
+    for (int j = FEW + lane; j < p.len[i]; j += 32) {
+      const int pg = p.free_pages[off + j];
+      row[j] = pg;
+      c.ref_count[pg] = 1;
+    }
   }
 }
 
@@ -392,11 +421,12 @@ __device__ __forceinline__ void fork_cell(const zs_kv_cache& c, const Plan& p, c
   if (old != -1) hold(c, old, -1);
 }
 
-__global__ void __launch_bounds__(PLAN_THREADS) kv_fork_plan_kernel(const zs_kv_cache c, Plan p, const int* src,
-                                                                    const int* dst, int n, int rows_here) {
-  __shared__ int s_warp[32], s_first[PLAN_SLOTS];
+__global__ void __launch_bounds__(PLAN_THREADS) kv_fork_plan_kernel(const zs_kv_cache c, const Plan plan,
+                                                                    const int* src, const int* dst, int n,
+                                                                    int rows_here) {
+  __shared__ PlanShared sh;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (c.max_seqs <= PLAN_SLOTS) p.first = s_first;
+  Plan p = in_shared(c, plan, n, sh);
   mark_first(dst, n, c.max_seqs, p.first);
   auto need_of = [&](int i) -> int {
     const int s = src[i], d = dst[i];
@@ -413,7 +443,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv_fork_plan_kernel(const zs_kv_
     p.len[i] = ok ? c.seq_lens[s] : 0;
     if (p.len[i] < 0 || p.len[i] > c.max_pages * c.page_size) record_error(ZS_DEVERR_INDEX);
   }
-  allot(c, p, n, need_of, s_warp);
+  allot(c, p, n, need_of, sh.warp, sh.free_pages);
   int moves = 0;
   for (int i0 = 0; i0 < n; i0 += PLAN_THREADS) {
     const int i = i0 + threadIdx.x;
@@ -424,7 +454,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv_fork_plan_kernel(const zs_kv_
       mv = false;
     }
     int sum;
-    const int at = moves + block_scan(mv ? 1 : 0, s_warp, &sum);
+    const int at = moves + block_scan(mv ? 1 : 0, sh.warp, &sum);
     if (mv) {
       p.from[at] = last;
       p.to[at] = p.free_pages[p.off[i]];
@@ -433,6 +463,11 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv_fork_plan_kernel(const zs_kv_
     moves += sum;
   }
   if (threadIdx.x == 0) *p.count = moves;
+  if (p.off != plan.off)
+    for (int i = threadIdx.x; i < n; i += PLAN_THREADS) plan.off[i] = p.off[i], plan.len[i] = p.len[i];
+  if (p.free_pages != plan.free_pages && !rows_here)
+    for (int i = threadIdx.x; i < n; i += PLAN_THREADS)
+      if (p.off[i] >= 0 && p.len[i] % c.page_size) plan.free_pages[p.off[i]] = p.free_pages[p.off[i]];
   if (!rows_here) return;
   for (int e = threadIdx.x; e < n * c.max_pages; e += PLAN_THREADS) {
     const int i = e / c.max_pages;
@@ -569,7 +604,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv_copy_plan_kernel(const zs_kv_
 enum { AFTER_COPY, AFTER_FORK, AFTER_COMPACT };
 
 template <int AFTER>
-__global__ void __launch_bounds__(256) kv_apply_kernel(const zs_kv_cache c, const Plan p, const int* dst, int n) {
+__global__ void __launch_bounds__(256, 8) kv_apply_kernel(const zs_kv_cache c, const Plan p, const int* dst, int n) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int64_t me = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, all = (int64_t)gridDim.x * blockDim.x;
   if (AFTER == AFTER_FORK) {
@@ -590,14 +625,14 @@ __global__ void __launch_bounds__(256) kv_apply_kernel(const zs_kv_cache c, cons
   }
   const int64_t run = (int64_t)c.page_size * c.head_dim / 8;        // 16-byte words of a whole run
   const int64_t page = run * c.n_kv_heads;
-  const int64_t slabs = 2 * (int64_t)c.n_layers;
-  const int64_t items = (int64_t)*p.count * slabs * c.n_kv_heads;
+  const int per = 2 * c.n_layers * c.n_kv_heads, count = *p.count;   // items of a move
   uint4* kv = reinterpret_cast<uint4*>(c.kv);
-  for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
-    const int64_t m = it / (slabs * c.n_kv_heads), rest = it - m * slabs * c.n_kv_heads;
-    const int64_t slab = rest / c.n_kv_heads, h = rest - slab * c.n_kv_heads;
-    const uint4* from = kv + (slab * c.num_pages + p.from[m]) * page + h * run;
-    uint4* to = kv + (slab * c.num_pages + p.to[m]) * page + h * run;
+  int m = blockIdx.x / per, rest = blockIdx.x % per;
+  const int dm = gridDim.x / per, dr = gridDim.x % per;
+  while (m < count) {
+    const int slab = rest / c.n_kv_heads, h = rest - slab * c.n_kv_heads;
+    const uint4* from = kv + (slab * (int64_t)c.num_pages + p.from[m]) * page + h * run;
+    uint4* to = kv + (slab * (int64_t)c.num_pages + p.to[m]) * page + h * run;
     const int words = p.rows[m] * (c.head_dim / 8);
     for (int w = threadIdx.x; w < words; w += 4 * 256) {
       uint4 v[4];
@@ -608,6 +643,9 @@ __global__ void __launch_bounds__(256) kv_apply_kernel(const zs_kv_cache c, cons
       for (int e = 0; e < 4; ++e)
         if (w + e * 256 < words) to[w + e * 256] = v[e];
     }
+    m += dm;
+    rest += dr;
+    if (rest >= per) rest -= per, ++m;
   }
 }
 

@@ -80,9 +80,13 @@ def sample(logits, temperature=0.0, generator=None):
 def generate(model, prompts, max_new_tokens, *, temperature=0.0, eos_token_id=None, page_size=64, generator=None):
     """Continuations (a list of lists of ids) of prompts (a list of non-empty id sequences).  Greedy
     by default; a sequence ends after eos_token_id (which is part of it) or max_new_tokens ids."""
-    prompts = [torch.as_tensor(p, dtype=torch.long).reshape(-1) for p in prompts]
+    prompts = [torch.as_tensor(p, dtype=torch.long).reshape(-1).cpu() for p in prompts]
     if not prompts or min(p.numel() for p in prompts) < 1:
         raise Z.ZsError("generate needs prompts of at least one token")
+    ids = torch.cat(prompts)
+    if int(ids.min()) < 0 or int(ids.max()) >= model.embedding.weight.size(0):
+        raise Z.ZsError(f"token ids must lie in [0, {model.embedding.weight.size(0)}) (got {int(ids.min())} to "
+                        f"{int(ids.max())})")
     if max_new_tokens < 1:
         return [[] for _ in prompts]
     dev = model.embedding.weight.device
@@ -96,7 +100,7 @@ def generate(model, prompts, max_new_tokens, *, temperature=0.0, eos_token_id=No
     cu = torch.zeros(len(prompts) + 1, dtype=torch.int32, device=dev)
     cu[1:] = n_new.cumsum(0)
     cache.extend(step.slots, n_new)
-    logits = model.forward_paged(torch.cat(prompts).to(dev), cache, cache.block_table, cache.seq_lens, cu)
+    logits = model.forward_paged(ids.to(dev), cache, cache.block_table, cache.seq_lens, cu)
     out = torch.full((len(prompts), max_new_tokens), -1, dtype=torch.long, device=dev)
     step.active.fill_(1)
     for i in range(max_new_tokens):

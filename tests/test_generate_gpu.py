@@ -162,4 +162,7 @@ def test_generate_refuses():
             m.generate(bad, 4)
     with pytest.raises(ZsError, match="positions"):
         m.generate([[1] * 500], 100)
+    for bad in ([[1, cfg.vocab_size]], [[1], [2, -1]]):
+        with pytest.raises(ZsError, match="token ids"):
+            m.generate(bad, 4)
     assert m.generate([[1, 2]], 0) == [[]]

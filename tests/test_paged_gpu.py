@@ -448,6 +448,44 @@ def test_large_tables():
     _same(c, ref)
 
 
+@pytest.mark.parametrize("n,M", [(1024, 4), (1024, 12), (1025, 4), (1025, 12), (300, 40), (1, 9000)])
+def test_many_requests(n, M):
+    """On both sides of a block's threads, of the cells that it rewrites itself and of the pages that it lists."""
+    S = 1100 if M < 100 else 8
+    c, ref = _cache(P=16000, page=16, slots=S, M=M, L=1, Hkv=1)
+    r = np.random.default_rng(n + M)
+    slots = [int(x) for x in r.permutation(S)[:n]]
+    for most in (16, 30, min(M, 20) * 16 - 46):
+        t = [int(x) for x in r.integers(0, most + 1, n)]
+        c.extend(slots, t), ref.extend(slots, t)
+        _same(c, ref)
+    src, dst = (slots if n > 1 else slots * 2), [int(x) for x in r.permutation(S)[:max(n, 2)]]
+    c.fork(src, dst), ref.fork(src, dst)
+    _same(c, ref)
+    c.fork(dst, src[:1] + dst[1:]), ref.fork(dst, src[:1] + dst[1:])
+    _same(c, ref)
+
+
+def test_lengths_below_zero_are_refused():
+    """A table that is not the cache's own: nothing is written before a row of the table."""
+    from zs_b200 import _lib as Z
+
+    c, _ = _cache()
+    c.extend([0, 1], [20, 20])
+    c.seq_lens[1] = -1000
+    before = c.meta.clone()
+    c.extend([1], [5])
+    assert torch.equal(c.meta, before) and Z.device_error() == 0x10
+    Z.clear_device_error()
+    c.fork([1], [2])
+    assert torch.equal(c.meta, before) and Z.device_error() == 0x10
+    Z.clear_device_error()
+    c.extend([0, 1], [30, 1])
+    assert c.seq_lens.tolist()[:2] == [50, -1000] and c.block_table[0, :4].min() >= 0
+    assert (c.block_table[1:] == before[:54].view(6, 9)[1:]).all()
+    Z.clear_device_error()
+
+
 def test_beam_permutation_and_check():
     from zs_b200 import ZsError
 
