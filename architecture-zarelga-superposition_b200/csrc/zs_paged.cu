@@ -310,24 +310,10 @@ __device__ __forceinline__ void hold(const zs_kv_cache& c, int page, int by) {
     record_error(ZS_DEVERR_INDEX);
 }
 
-// Up to PLAN_THREADS requests keep their part of the plan in shared memory: what the block
-// writes and reads again would otherwise be a trip to L2 each time.  The counts, which it
-// searches in the end, are asked for at its start.
-struct PlanShared {
-  int warp[32], first[PLAN_SLOTS], off[PLAN_THREADS], len[PLAN_THREADS], free_pages[PLAN_THREADS];
-};
-__device__ __forceinline__ Plan in_shared(const zs_kv_cache& c, Plan p, int n, PlanShared& s) {
-  if (c.max_seqs <= PLAN_SLOTS) p.first = s.first;
-  if (n <= PLAN_THREADS) p.off = s.off, p.len = s.len;
-  if ((int64_t)threadIdx.x * 32 < c.num_pages)
-    asm volatile("prefetch.global.L1 [%0];" ::"l"(c.ref_count + threadIdx.x * 32));
-  return p;
-}
-
 // Each request's number of new pages (need_of(i), -1: refused) scanned in
 // order into plan.off; the pages found; requests past them refused.
 template <typename F>
-__device__ __forceinline__ void allot(const zs_kv_cache& c, Plan& p, int n, F need_of, int* s_warp, int* s_free) {
+__device__ __forceinline__ void allot(const zs_kv_cache& c, const Plan& p, int n, F need_of, int* s_warp) {
   int total = 0;
   for (int i0 = 0; i0 < n; i0 += PLAN_THREADS) {
     const int i = i0 + threadIdx.x;
@@ -341,7 +327,6 @@ __device__ __forceinline__ void allot(const zs_kv_cache& c, Plan& p, int n, F ne
   }
   __syncthreads();
   const int want = total > (int)c.num_pages ? (int)c.num_pages : total;
-  if (want <= PLAN_THREADS) p.free_pages = s_free;
   const int have = find_free(c.ref_count, c.num_pages, want, p.free_pages, s_warp);
   for (int i = threadIdx.x; i < n; i += PLAN_THREADS) {
     const int need = need_of(i);
@@ -353,10 +338,10 @@ __device__ __forceinline__ void allot(const zs_kv_cache& c, Plan& p, int n, F ne
   __syncthreads();
 }
 
-__global__ void __launch_bounds__(PLAN_THREADS) kv_extend_kernel(const zs_kv_cache c, const Plan plan,
+__global__ void __launch_bounds__(PLAN_THREADS) kv_extend_kernel(const zs_kv_cache c, Plan p,
                                                                  const int* slots, const int* tokens, int n) {
-  __shared__ PlanShared sh;
-  Plan p = in_shared(c, plan, n, sh);
+  __shared__ int s_warp[32], s_first[PLAN_SLOTS];
+  if (c.max_seqs <= PLAN_SLOTS) p.first = s_first;
   mark_first(slots, n, c.max_seqs, p.first);
   auto need_of = [&](int i) -> int {
     const int s = slots[i], t = tokens[i];
@@ -373,7 +358,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv_extend_kernel(const zs_kv_cac
     else if ((int64_t)c.seq_lens[s] + t > (int64_t)c.max_pages * c.page_size)
       record_error(ZS_DEVERR_CACHE_FULL);
   }
-  allot(c, p, n, need_of, sh.warp, sh.free_pages);
+  allot(c, p, n, need_of, s_warp);
   // A thread writes a request's first pages, a warp the many of a prompt.
   constexpr int FEW = 2;
   for (int i = threadIdx.x; i < n; i += PLAN_THREADS) {
@@ -421,12 +406,12 @@ __device__ __forceinline__ void fork_cell(const zs_kv_cache& c, const Plan& p, c
   if (old != -1) hold(c, old, -1);
 }
 
-__global__ void __launch_bounds__(PLAN_THREADS) kv_fork_plan_kernel(const zs_kv_cache c, const Plan plan,
+__global__ void __launch_bounds__(PLAN_THREADS) kv_fork_plan_kernel(const zs_kv_cache c, Plan p,
                                                                     const int* src, const int* dst, int n,
                                                                     int rows_here) {
-  __shared__ PlanShared sh;
+  __shared__ int s_warp[32], s_first[PLAN_SLOTS];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  Plan p = in_shared(c, plan, n, sh);
+  if (c.max_seqs <= PLAN_SLOTS) p.first = s_first;
   mark_first(dst, n, c.max_seqs, p.first);
   auto need_of = [&](int i) -> int {
     const int s = src[i], d = dst[i];
@@ -443,7 +428,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv_fork_plan_kernel(const zs_kv_
     p.len[i] = ok ? c.seq_lens[s] : 0;
     if (p.len[i] < 0 || p.len[i] > c.max_pages * c.page_size) record_error(ZS_DEVERR_INDEX);
   }
-  allot(c, p, n, need_of, sh.warp, sh.free_pages);
+  allot(c, p, n, need_of, s_warp);
   int moves = 0;
   for (int i0 = 0; i0 < n; i0 += PLAN_THREADS) {
     const int i = i0 + threadIdx.x;
@@ -454,7 +439,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv_fork_plan_kernel(const zs_kv_
       mv = false;
     }
     int sum;
-    const int at = moves + block_scan(mv ? 1 : 0, sh.warp, &sum);
+    const int at = moves + block_scan(mv ? 1 : 0, s_warp, &sum);
     if (mv) {
       p.from[at] = last;
       p.to[at] = p.free_pages[p.off[i]];
@@ -463,11 +448,6 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv_fork_plan_kernel(const zs_kv_
     moves += sum;
   }
   if (threadIdx.x == 0) *p.count = moves;
-  if (p.off != plan.off)
-    for (int i = threadIdx.x; i < n; i += PLAN_THREADS) plan.off[i] = p.off[i], plan.len[i] = p.len[i];
-  if (p.free_pages != plan.free_pages && !rows_here)
-    for (int i = threadIdx.x; i < n; i += PLAN_THREADS)
-      if (p.off[i] >= 0 && p.len[i] % c.page_size) plan.free_pages[p.off[i]] = p.free_pages[p.off[i]];
   if (!rows_here) return;
   for (int e = threadIdx.x; e < n * c.max_pages; e += PLAN_THREADS) {
     const int i = e / c.max_pages;
