@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(128, 7) paged_append_kernel(const AppendArgs a
 //
 // The plan kernels run in one block: requests are served in order and take the
 // lowest-numbered free pages, so every result is a function of the tables
-// alone.  Page data moves in copy_pages_kernel, which reads the plan's list of
+// alone.  Page data moves in kv_apply_kernel, which reads the plan's list of
 // (from, to, rows); the lists name free pages as targets only, so no copy
 // reads what another writes.
 
@@ -359,7 +359,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv_extend_kernel(const zs_kv_cac
       record_error(ZS_DEVERR_CACHE_FULL);
   }
   allot(c, p, n, need_of, s_warp);
-  // A thread writes a request's first pages, a warp the many of a prompt.
+  // A thread writes a request's first pages, a warp the many of a prompt (a warp for every request: 64 slots
+  // by a token 6.4 us instead of 4.4, 1000 slots 33 instead of 10).
   constexpr int FEW = 2;
   for (int i = threadIdx.x; i < n; i += PLAN_THREADS) {
     const int off = p.off[i];
@@ -580,7 +581,10 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv_copy_plan_kernel(const zs_kv_
 // What follows a plan: the tables rewritten (FORK: the new rows; COMPACT: moved pages
 // renamed), then the page data.  One work item: one head's filled rows of one page of one
 // layer's keys or values, a contiguous run of rows * hd elements.  HBM-bound: read once,
-// written once.  Launched while the plan still runs; waits for its end.
+// written once.  Launched while the plan still runs; waits for its end.  Eight blocks of 32
+// registers an SM, all resident, no division per item (five of 48 registers with 64-bit divisions: fork of 32 beams
+// over 16 layers 21.6 us instead of 20.9; about 10 of them do not grow with the bytes, the rest
+// moves at 6.5 TB/s).  Compaction of 48 sequences in 8 layers: 136 us, 5.5 TB/s.
 enum { AFTER_COPY, AFTER_FORK, AFTER_COMPACT };
 
 template <int AFTER>
