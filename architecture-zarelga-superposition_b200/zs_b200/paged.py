@@ -74,7 +74,8 @@ def paged_prompt_attention(q, k_pages, v_pages, block_table, seq_lens, cu_seqlen
     sequence (the last `window` of them), key head h // (H // Hkv), scale 1/sqrt(hd) by default.
     k_sink [H, hd]: one more logit q . k_sink per head whose value is zero.  gate [T, H] (q's dtype;
     a strided view will do): o is multiplied by sigmoid(gate).  Rows that see no key, and rows
-    outside every sequence, are zero.  At most 128 query heads share a key head."""
+    outside every sequence, are zero.  At most 128 query heads share a key head.  A value that is NaN or
+    infinite reaches no other sequence, but may reach earlier rows of its own (zero times it)."""
     if cu_seqlens is None:
         _fail("cu_seqlens is required")
     Z.INSTR.launches += 2
