@@ -1608,7 +1608,9 @@ static int attn_args(paged::AttnArgs& a, const void* q, int64_t ldq, const void*
   a.Hkv = Hkv;
   a.page = page;
   a.window = window;
-  a.scale_log2 = scale * 1.4426950408889634f;
+  // At least the smallest normal number, which makes every finite logit next to nothing as a scale of zero does:
+  // masked scores are -inf before they are scaled, and -inf * 0 is NaN.
+  a.scale_log2 = fmaxf(scale * 1.4426950408889634f, 1.17549435e-38f);
   a.k_sink = k_sink;
   a.gate = gate;
   a.ldg = ldg;
