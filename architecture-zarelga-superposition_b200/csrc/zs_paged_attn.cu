@@ -1306,8 +1306,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
       if (!ok) break;
       if (a.k_sink != nullptr && loaded) {
         // Q K_sink^T by mma.sync, 16 rows by 8 heads at a time, from which each row takes its own head's
-        // column; the f32 sink as the sum of two values of Q's type (2^-17 of it is lost).  Little code:
-        // what runs once a part is fetched anew each time, a few cycles an instruction.
+        // column; the f32 sink as the sum of two values of Q's type (2^-17 of it is lost in bf16, 2^-22 in
+        // f16), which f16 has the range for once a head's sink is brought to below 2^14 by a power of two.
+        // Little code: what runs once a part is fetched anew each time, a few cycles an instruction.
         ok = warp_wait(&z_free[t], (z_n++ & 1) ^ 1, s_abort, ZS_DEVERR_TIMEOUT_EPILOGUE);
         if (!ok) break;
         const uint32_t qt = smem_u32(smem + L::OFF_Q + t * L::TILE);
@@ -1316,11 +1317,29 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
         for (int g0 = 0; g0 < G; g0 += 8) {
           uint32_t hi[HD / 16][2], lo[HD / 16][2];
           const float* sink = a.k_sink + (int64_t)(b.hk * G + min(g0 + r4, G - 1)) * HD + c4 * 2;
+          float up = 1.f, down[2] = {1.f, 1.f};          // the power of two; its inverse for this lane's columns
+          if (std::is_same<T, __half>::value) {
+            float big = 0.f;
+#pragma unroll
+            for (int kk = 0; kk < HD / 8; ++kk) {
+              const float2 f = __ldg(reinterpret_cast<const float2*>(sink + kk * 8));
+              big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
+            }
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+            const int e = min(267 - (__float_as_int(big) >> 23), 253);
+            up = __int_as_float(e << 23);
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+              down[x] = __shfl_sync(0xffffffffu, __int_as_float((254 - e) << 23), (c4 * 2 + x) * 4);
+          }
 #pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              const float2 f = __ldg(reinterpret_cast<const float2*>(sink + kk * 16 + x * 8));
+              float2 f = __ldg(reinterpret_cast<const float2*>(sink + kk * 16 + x * 8));
+              f.x *= up;
+              f.y *= up;
               const typename Pair<T>::type h2 = Pair<T>::from_f(f.x, f.y);
               const float2 g2 = Pair<T>::to_f(h2);
               const typename Pair<T>::type l2 = Pair<T>::from_f(f.x - g2.x, f.y - g2.y);
@@ -1342,7 +1361,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
               const int r = r0 + r4 + x * 8, g = r - (r * inv >> 16) * G - g0;
-              if (g >> 1 == c4) s_z[t * PT_ROWS + r] = g & 1 ? acc[x * 2 + 1] : acc[x * 2];
+              if (g >> 1 == c4) s_z[t * PT_ROWS + r] = g & 1 ? acc[x * 2 + 1] * down[1] : acc[x * 2] * down[0];
             }
           }
         }
