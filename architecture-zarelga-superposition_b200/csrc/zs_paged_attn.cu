@@ -7,6 +7,7 @@
 // sigmoid gate on o.  A row that sees no key is zero, its log-sum-exp the sink
 // logit or -inf.
 #include "zs_common.cuh"
+#include "zs_paged_plan.cuh"
 
 #include <atomic>
 #include <type_traits>
@@ -42,7 +43,7 @@ struct AttnArgs {
 __device__ __forceinline__ int cut_length(const AttnArgs& a, int seq) {
   const int len = __ldg(a.seq_lens + seq), cap = a.max_pages * a.page;
   if (len > cap) record_error(ZS_DEVERR_INDEX);
-  return len > cap ? cap : len;
+  return length_within(len, cap);
 }
 
 // ------------------------------------------------------------------------ decode
@@ -130,8 +131,7 @@ struct Span {              // the key tiles of a sequence
 template <int TILE>
 __device__ __forceinline__ Span span_of(const AttnArgs& a, int seq) {
   Span s;
-  const int len = cut_length(a, seq);
-  s.len = len > 0 ? len : 0;
+  s.len = cut_length(a, seq);
   s.first_key = a.window > 0 && s.len > a.window ? s.len - a.window : 0;
   s.first_tile = s.first_key / TILE;
   // an empty sequence has one tile with no key in it, so that its rows are written
@@ -831,13 +831,12 @@ __device__ __forceinline__ PromptBlock block_at(const AttnArgs& a, int seq, int 
   b.left = n - skip;
   b.len = cut_length(a, seq);
   b.pos0 = b.len - n + skip;
-  b.floor = a.window > 0 ? max(b.len - n - (a.window - 1), 0) : 0;
+  b.floor = first_seen(b.len - n, a.window);
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
-    const int rows = min(b.left - t * tpt, tpt);         // tokens of the tile
-    const int p0 = b.pos0 + t * tpt, p1 = p0 + rows - 1;
-    b.lo[t] = (a.window > 0 ? max(p0 - (a.window - 1), 0) : 0) / PT_KEYS;
-    b.cnt[t] = rows > 0 && p1 >= 0 ? p1 / PT_KEYS - b.lo[t] + 1 : 0;
+    const KeyTiles k = key_tiles<PT_KEYS>(b.pos0 + t * tpt, min(b.left - t * tpt, tpt), a.window);
+    b.lo[t] = k.lo;
+    b.cnt[t] = k.cnt;
   }
   b.first = b.cnt[0] > 0 ? b.lo[0] : b.lo[1];
   const int end = b.cnt[1] > 0 ? b.lo[1] + b.cnt[1] : b.lo[0] + b.cnt[0];
@@ -1652,7 +1651,7 @@ static int attn_args(paged::AttnArgs& a, const void* q, int64_t ldq, const void*
   a.H = H;
   a.Hkv = Hkv;
   a.page = page;
-  a.window = window;
+  a.window = paged::window_within(window, (int64_t)max_pages * page);
   // At least the smallest normal number, which makes every finite logit next to nothing as a scale of zero does:
   // masked scores are -inf before they are scaled, and -inf * 0 is NaN.
   a.scale_log2 = fmaxf(scale * 1.4426950408889634f, 1.17549435e-38f);
