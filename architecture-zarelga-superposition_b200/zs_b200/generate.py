@@ -15,8 +15,8 @@ from .dense import one_group_routing
 
 class DecodeStep:
     """One decode step of all slots of a cache as a CUDA graph: the slots grow by `active` (0 or 1)
-    tokens, `tokens` go in, `logits` come out.  An inactive slot's row is computed and ignored; its
-    newest token's keys are overwritten, so it must not be continued later.
+    tokens, `tokens` go in, `logits` come out.  A slot that does not grow (inactive, or refused for want
+    of a page or of room) keeps what it holds and may go on later; its row of the logits means nothing.
 
     The recorded kernels read the weights' bf16 shadows where they lay at the recording.  The
     package's optimizer writes those with the weights; after any other change of a weight (a
@@ -34,8 +34,12 @@ class DecodeStep:
 
     def _run(self):
         c = self.cache
+        before = c.seq_lens.clone()
         c.extend(self.slots, self.active)
-        return self.model.forward_paged(self.tokens, c, c.block_table, c.seq_lens)
+        # a slot that did not grow has no new token: with a length of zero nothing is stored for it (its
+        # last position holds a token, maybe on a page that it shares) and nothing is read
+        lens = c.seq_lens * (c.seq_lens > before)
+        return self.model.forward_paged(self.tokens, c, c.block_table, lens)
 
     @staticmethod
     def _place(p):

@@ -167,7 +167,9 @@ class PagedKVCache:
 
     def extend(self, slots, n_tokens):
         """Slot slots[i] grows by n_tokens[i] >= 0 tokens, with pages for them; what they hold is
-        up to the caller (paged_append).  A slot named twice grows by its first request only."""
+        up to the caller (paged_append).  A slot named twice grows by its first request only.  A refused
+        slot has not grown, and tokens stored at its last positions would replace those that it holds:
+        compare seq_lens with a copy from before the call, or check(), before storing."""
         self._call(0, 1, slots, n_tokens)
 
     def fork(self, src, dst):
