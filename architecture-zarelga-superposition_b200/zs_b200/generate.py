@@ -7,6 +7,9 @@ since the launches would cost more than the work.
 """
 from __future__ import annotations
 
+import itertools
+import operator
+
 import torch
 
 from . import _lib as Z
@@ -18,9 +21,11 @@ class DecodeStep:
     tokens, `tokens` go in, `logits` come out.  A slot that does not grow (inactive, or refused for want
     of a page or of room) keeps what it holds and may go on later; its row of the logits means nothing.
 
-    The recorded kernels read the weights' bf16 shadows where they lay at the recording.  The
-    package's optimizer writes those with the weights; after any other change of a weight (a
-    torch operation, load_state_dict, another parameter in its place) the step is recorded again."""
+    The recorded kernels read the weights' bf16 shadows, the parameters and the buffers where they lay at the
+    recording.  The package's optimizer writes those in place; after any other change (of a weight by a
+    torch operation or load_state_dict; another tensor, parameter, buffer or module in the place of one;
+    another `model`, `cache`, `slots`, `active` or `tokens`) the step is recorded again.  Changes that no
+    tensor or module shows (a flag, a hook) need `graph = None`."""
 
     def __init__(self, model, cache):
         dev = cache.kv.device
@@ -42,13 +47,30 @@ class DecodeStep:
         return self.model.forward_paged(self.tokens, c, c.block_table, lens)
 
     @staticmethod
-    def _place(p):
-        """Where a kernel reads parameter p, and the change by torch that its shadow is in step with."""
-        sh = getattr(p, "_zs_sh", None)
-        return p.data_ptr(), None if sh is None else (sh.data_ptr(), p._version)
+    def _place(t):
+        """Where a kernel reads tensor t, and the change by torch that its shadow is in step with."""
+        sh = getattr(t, "_zs_sh", None)
+        return t.data_ptr(), None if sh is None else (sh.data_ptr(), t._version)
+
+    def _own(self):
+        return self.model, self.cache, self.slots, self.active, self.tokens
+
+    def _remember(self):
+        """What the recorded kernels depend on: this object's inputs and every module's modules, parameters and
+        buffers by identity, every tensor by its place.  The tensors' memory is held, so an address stands for it."""
+        self._inputs = self._own()
+        dicts = [d for m in self.model.modules() for d in (m._modules, m._parameters, m._buffers)]
+        values = [v for d in dicts for v in d.values()]
+        tensors = [v for v in values if torch.is_tensor(v)]
+        self._read = dicts, [len(d) for d in dicts], values, tensors, [self._place(t) for t in tensors]
+        self._memory = [(t.detach(), getattr(t, "_zs_sh", None)) for t in tensors]
 
     def _current(self):
-        return all(held.get(name) is p and self._place(p) == place for held, name, p, place in self._read)
+        # 0.15 ms of host time for 16 layers (357 modules), beside 2.3 ms of kernels for 64 slots
+        dicts, lens, values, tensors, places = self._read
+        return (all(map(operator.is_, self._own(), self._inputs)) and list(map(len, dicts)) == lens
+                and all(map(operator.is_, itertools.chain.from_iterable(d.values() for d in dicts), values))
+                and list(map(self._place, tensors)) == places)
 
     def __call__(self):
         if self.graph is not None and self._current():
@@ -64,10 +86,9 @@ class DecodeStep:
             torch.cuda.current_stream().synchronize()
             graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(graph):
-                self._static = self._run()
-        self._read = [(m._parameters, name, p, self._place(p)) for m in self.model.modules()
-                      for name, p in m._parameters.items() if p is not None]
-        self.graph = graph
+                static = self._run()
+        self._remember()
+        self.graph, self._static = graph, static
         return self.logits
 
 

@@ -1,6 +1,7 @@
 """DecodeStep: what a recorded step leaves alone, and when it is recorded again."""
 import pytest
 import torch
+import torch.nn as nn
 
 from test_generate_gpu import _model
 
@@ -83,3 +84,94 @@ def test_a_step_that_finds_no_page_changes_no_token():
         assert torch.equal(_seq(c, 0), was)
         with pytest.raises(ZsError, match="no free page"):
             c.check()
+
+
+def _sparse_model():
+    """Two of eight routed experts a token."""
+    from modeling.model_config import ModelConfig
+    from zs_b200.lm import MoELM
+
+    cfg = ModelConfig(vocab_size=1024, embed_size=256, hidden_size=256, transformer_depth=3, intermediate_size=256,
+                      n_experts=9, n_shared_experts=1, n_experts_per_token=2, n_attention_heads=4,
+                      n_key_value_heads=2, attention_window_pattern=(None, 40, None), max_position_embeddings=512,
+                      sequence_length=512, pos_rope_dims=32, attention_sink=True, use_qk_norm=True)
+    torch.manual_seed(0)
+    return cfg, MoELM(cfg).cuda()
+
+
+def _other_linear(m, cfg):
+    new = nn.Linear(cfg.hidden_size, cfg.vocab_size, bias=False, device="cuda")
+    m.output_layer = new
+
+
+def _other_block(m, cfg):
+    _, n = _sparse_model()
+    n.layers[1].self_attn.q_proj.weight.data.mul_(-1)
+    m.layers[1] = n.layers[1]
+
+
+def _other_gate_bias(m, cfg):
+    b = m.layers[0].mlp.gate.expert_biases
+    m.layers[0].mlp.gate.expert_biases = torch.arange(b.numel(), device="cuda", dtype=b.dtype)
+
+
+def _other_rotation(m, cfg):
+    att = m.layers[2].self_attn
+    att.pos_cos_cache, att.pos_sin_cache = att.pos_sin_cache.clone(), att.pos_cos_cache.clone()
+
+
+def _sink_removed(m, cfg):
+    m.layers[0].self_attn.k_sink = None
+
+
+def _fewer_layers(m, cfg):
+    del m.layers[2]
+
+
+def _other_tokens(m, cfg, step):
+    step.tokens = step.tokens + 100
+
+
+def _back_at_the_old_address(m, cfg):
+    w = m.output_layer.weight
+    w.data = w.data * 2
+    w.data = w.data * 3                                      # may lie where the first one lay
+
+
+CHANGES = [_other_linear, _other_block, _other_gate_bias, _other_rotation, _sink_removed, _fewer_layers,
+           _other_tokens, _back_at_the_old_address]
+
+
+@pytest.mark.parametrize("change", CHANGES, ids=lambda f: f.__name__[1:])
+def test_a_recorded_step_follows_its_modules_and_buffers(change):
+    from zs_b200.generate import DecodeStep
+
+    cfg, m = _sparse_model()
+    c = m.new_cache(2, 64, page_size=16)
+    step = DecodeStep(m, c)
+    step.active.fill_(1)
+    step.tokens.copy_(torch.tensor([3, 9]))
+    for _ in range(3):
+        step()
+    recorded = step.graph
+    step()
+    assert step.graph is recorded
+    meta, kv = c.meta.clone(), c.kv.clone()
+    old = step().clone()
+    c.meta.copy_(meta)
+    c.kv.copy_(kv)
+    with torch.no_grad():
+        change(m, cfg, *([step] if change is _other_tokens else []))
+    changed = False
+    for k in range(3):                                       # recorded anew, then replayed
+        got = step().clone()
+        assert step.graph is not recorded
+        c.meta.copy_(meta)
+        c.kv.copy_(kv)
+        c.extend(step.slots, step.active)
+        want = m.forward_paged(step.tokens, c, c.block_table, c.seq_lens)
+        assert torch.equal(got, want)
+        changed |= not torch.equal(got, old)
+        meta, kv = c.meta.clone(), c.kv.clone()
+    assert changed
+    c.check()
