@@ -139,17 +139,22 @@ class MoELM(nn.Module):
         """Logits [num_seqs, vocab] after each sequence's last new token.  ids [T]: the packed new
         tokens; cache: a PagedKVCache whose slots already count them (PagedKVCache.extend);
         block_table, seq_lens: the rows of the cache's tables that belong to the sequences;
-        cu_seqlens [num_seqs + 1]: their rows in ids (None: one new token each).  Runs under bf16
-        autocast whatever the caller's context."""
+        cu_seqlens [num_seqs + 1]: their rows in ids (None: one new token each).  A sequence without new
+        tokens gets a row of zeros.  Runs under bf16 autocast whatever the caller's context."""
         from .dense import dense_linear
 
+        if ids.numel() == 0 and (cu_seqlens is not None or block_table.size(0) == 0):
+            head = self.output_layer.weight
+            return torch.zeros(block_table.size(0), head.size(0), dtype=torch.bfloat16, device=head.device)
         with torch.autocast("cuda", dtype=torch.bfloat16, cache_enabled=False):
             h = self.embed(ids.view(1, -1))
             for i, block in enumerate(self.layers):
                 h = block.forward_paged(h, *cache.layer(i), block_table, seq_lens, cu_seqlens)
             h = self.final_norm(h)[0]
             if cu_seqlens is not None:
-                h = h.index_select(0, (cu_seqlens[1:] - 1).clamp_min(0).long())
+                # the row before an empty sequence's is another one's
+                rows = (cu_seqlens[1:] - 1).clamp_min(0).long()
+                h = h.index_select(0, rows).masked_fill((cu_seqlens[1:] <= cu_seqlens[:-1]).unsqueeze(1), 0)
             return dense_linear(h, [self.output_layer.weight], tag="logits")
 
     def new_cache(self, max_seqs, max_tokens, *, num_pages=None, page_size=64):

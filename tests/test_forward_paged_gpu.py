@@ -1,0 +1,36 @@
+"""MoELM.forward_paged and new_cache at their edges."""
+import pytest
+import torch
+
+from _util import rel_err
+from test_generate_gpu import TOL, _logits, _model
+
+pytestmark = pytest.mark.gpu
+
+
+def test_a_sequence_without_new_tokens_gets_no_other_ones_logits():
+    cfg, m = _model()
+    g = torch.Generator(device="cuda").manual_seed(1)
+    seqs = [torch.randint(0, cfg.vocab_size, (n,), device="cuda", generator=g) for n in (30, 21, 40, 18)]
+    c = m.new_cache(4, 128, page_size=16)
+    slots = torch.arange(4, dtype=torch.int32, device="cuda")
+
+    def run(parts):
+        n = torch.tensor([p.numel() for p in parts], dtype=torch.int32, device="cuda")
+        cu = torch.cat([n.new_zeros(1), n.cumsum(0).int()])
+        c.extend(slots, n)
+        return m.forward_paged(torch.cat(parts), c, c.block_table, c.seq_lens, cu)
+
+    none = seqs[0][:0]
+    run([none, seqs[1], none, seqs[3]])
+    was = c.kv.clone()
+    got = run([seqs[0], none, seqs[2], none])
+    for i in (0, 2):
+        assert rel_err(got[i], _logits(m, seqs[i])[-1]) < TOL
+    assert (got[1] == 0).all() and (got[3] == 0).all()
+    for s in (1, 3):                                         # and their tokens stay
+        ids = c.block_table[s, :2].long()
+        assert torch.equal(c.kv[:, :, ids], was[:, :, ids])
+    got = run([none, none, none, none])
+    assert got.shape == (4, cfg.vocab_size) and (got == 0).all()
+    c.check()
