@@ -140,7 +140,8 @@ class MoELM(nn.Module):
         tokens; cache: a PagedKVCache whose slots already count them (PagedKVCache.extend);
         block_table, seq_lens: the rows of the cache's tables that belong to the sequences;
         cu_seqlens [num_seqs + 1]: their rows in ids (None: one new token each).  A sequence without new
-        tokens gets a row of zeros.  Runs under bf16 autocast whatever the caller's context."""
+        tokens gets a row of zeros; rows behind the last token there is are not read.  Runs under
+        bf16 autocast whatever the caller's context."""
         from .dense import dense_linear
 
         if ids.numel() == 0 and (cu_seqlens is not None or block_table.size(0) == 0):
@@ -152,8 +153,8 @@ class MoELM(nn.Module):
                 h = block.forward_paged(h, *cache.layer(i), block_table, seq_lens, cu_seqlens)
             h = self.final_norm(h)[0]
             if cu_seqlens is not None:
-                # the row before an empty sequence's is another one's
-                rows = (cu_seqlens[1:] - 1).clamp_min(0).long()
+                # the row before an empty sequence's is another one's; a row that is not there is none to ask for
+                rows = (cu_seqlens[1:] - 1).clamp(0, h.size(0) - 1).long()
                 h = h.index_select(0, rows).masked_fill((cu_seqlens[1:] <= cu_seqlens[:-1]).unsqueeze(1), 0)
             return dense_linear(h, [self.output_layer.weight], tag="logits")
 

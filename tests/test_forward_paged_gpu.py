@@ -34,3 +34,17 @@ def test_a_sequence_without_new_tokens_gets_no_other_ones_logits():
     got = run([none, none, none, none])
     assert got.shape == (4, cfg.vocab_size) and (got == 0).all()
     c.check()
+
+
+def test_rows_beyond_the_tokens_are_not_read():
+    """cu_seqlens that count more rows than there are: no row outside the call's is asked for."""
+    from zs_b200 import _lib as Z
+
+    cfg, m = _model(layers=1, windows=(None,))
+    c = m.new_cache(2, 64, page_size=16)
+    c.extend([0, 1], [8, 50])
+    ids = torch.randint(0, cfg.vocab_size, (20,), device="cuda", generator=torch.Generator(device="cuda").manual_seed(0))
+    cu = torch.tensor([0, 8, 58], dtype=torch.int32, device="cuda")
+    got = m.forward_paged(ids, c, c.block_table, c.seq_lens, cu)
+    assert rel_err(got[0], _logits(m, ids[:8])[-1]) < TOL
+    assert torch.isfinite(got).all() and Z.device_error() == 0
