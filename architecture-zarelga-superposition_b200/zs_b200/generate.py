@@ -119,7 +119,7 @@ def generate(model, prompts, max_new_tokens, *, temperature=0.0, eos_token_id=No
     longest = max(lens) + max_new_tokens
     if longest > model.config.max_position_embeddings:
         raise Z.ZsError(f"{longest} positions exceed the model's {model.config.max_position_embeddings}")
-    cache = model.new_cache(len(prompts), longest, page_size=page_size)
+    cache = model.new_cache(len(prompts), longest, page_size=page_size, num_pages=len(prompts) * -(-longest // page_size))
     step = DecodeStep(model, cache)
     n_new = torch.tensor(lens, dtype=torch.int32, device=dev)
     cu = torch.zeros(len(prompts) + 1, dtype=torch.int32, device=dev)

@@ -160,13 +160,14 @@ class MoELM(nn.Module):
 
     def new_cache(self, max_seqs, max_tokens, *, num_pages=None, page_size=64):
         """A PagedKVCache for this model: max_seqs slots of up to max_tokens tokens, in num_pages
-        pages (by default enough for all slots to be full)."""
+        pages (by default enough for all slots to be full, and one more each: PagedKVCache.fork takes
+        its new pages before it lets the old ones go)."""
         from .paged import PagedKVCache
 
         att = self.layers[0].self_attn
         per_seq = -(-max_tokens // page_size)
         return PagedKVCache(len(self.layers), att.num_key_value_heads, att.head_dim,
-                            num_pages=num_pages or max_seqs * per_seq, page_size=page_size, max_seqs=max_seqs,
+                            num_pages=num_pages or max_seqs * (per_seq + 1), page_size=page_size, max_seqs=max_seqs,
                             max_pages_per_seq=per_seq, device=self.embedding.weight.device)
 
     def generate(self, prompts, max_new_tokens, **options):

@@ -175,7 +175,8 @@ class PagedKVCache:
     def fork(self, src, dst):
         """Slot dst[i] becomes a copy of slot src[i] as it was before the call (beam search:
         fork(parents, slots)); what dst[i] held is let go.  Whole pages are shared; the filled
-        rows of a last partial page are copied into a page of dst[i]'s own."""
+        rows of a last partial page are copied into a page of dst[i]'s own, which has to be free
+        before the call (a pool with a page to spare for every slot always has one)."""
         self._call(1, 2, src, dst)
 
     def free(self, slots):

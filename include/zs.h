@@ -732,7 +732,8 @@ int zs_paged_decode_attention(const void* q, int64_t ldq, const void* k_pages, c
  *   zs_kv_extend: slots[i] grows by tokens[i] >= 0 tokens, with pages for them.
  *   zs_kv_fork: dst[i] becomes a copy of src[i] as it was before the call (what
  *     dst[i] held is let go; src[i] == dst[i] stays): whole pages are shared, the
- *     rows of a last partial page are copied into a free page.
+ *     rows of a last partial page are copied into a page that is free before the
+ *     call.
  *   zs_kv_free: slots become empty; pages that no row holds are free.
  *   zs_kv_compact: the pages in use become pages 0 .. U-1: the k-th free page
  *     below U takes the k-th used page from U on.

@@ -48,3 +48,25 @@ def test_rows_beyond_the_tokens_are_not_read():
     got = m.forward_paged(ids, c, c.block_table, c.seq_lens, cu)
     assert rel_err(got[0], _logits(m, ids[:8])[-1]) < TOL
     assert torch.isfinite(got).all() and Z.device_error() == 0
+
+
+def test_a_default_cache_forks_between_full_slots():
+    """Every slot holds as many tokens as it may, none shares a page: each takes over another one's sequence."""
+    cfg, m = _model(layers=1, windows=(None,))
+    c = m.new_cache(3, 40, page_size=16)
+    slots = torch.arange(3, dtype=torch.int32, device="cuda")
+    c.extend(slots, torch.tensor([40, 39, 33], dtype=torch.int32, device="cuda"))
+    c.kv.copy_(torch.randn(c.kv.shape, device="cuda"))
+
+    def held(s):
+        n = int(c.seq_lens[s])
+        x = c.kv[:, :, c.block_table[s, :-(-n // 16)].long()].transpose(2, 3)
+        return x.reshape(*x.shape[:3], -1, x.size(-1))[..., :n, :].clone()
+
+    was = [held(s) for s in range(3)]
+    for _ in range(5):                                       # the pages let go serve the next fork
+        c.fork([1, 2, 0], [0, 1, 2])
+        c.check()
+        was = [was[1], was[2], was[0]]
+        for s in range(3):
+            assert torch.equal(held(s), was[s])
