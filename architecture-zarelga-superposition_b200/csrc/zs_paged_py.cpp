@@ -373,4 +373,12 @@ PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_paged", "Paged key-value cach
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__paged(void) { return PyModule_Create(&module_def); }
+// abi: the Python and torch that this was compiled against, which paged.py compares before the first call.
+PyMODINIT_FUNC PyInit__paged(void) {
+  PyObject* m = PyModule_Create(&module_def);
+  if (m != nullptr && PyModule_AddStringConstant(m, "abi", ZS_BINDING_ABI) < 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

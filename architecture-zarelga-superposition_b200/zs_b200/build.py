@@ -3,7 +3,8 @@
 The library is a plain shared object: no torch headers, no Python API.  It is
 written next to this file so it travels with the source tree.  Beside it
 _paged.so, a small host-only binding of the paged cache operators to CPython and
-torch, is compiled with g++ and linked against it.
+torch, is compiled with g++ and linked against it; _paged.so.abi names the Python and
+torch that it fits (it says so itself, too, when it is loaded).
 """
 from __future__ import annotations
 
@@ -19,6 +20,7 @@ CSRC = ROOT / "csrc"
 INCLUDE = ROOT.parent / "include"
 LIB = PKG / "libzs.so"
 BINDING = PKG / "_paged.so"
+BINDING_ABI = PKG / "_paged.so.abi"     # what BINDING was compiled against
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -46,8 +48,16 @@ def needs_build() -> bool:
     return any(p.stat().st_mtime > t for p in sources())
 
 
+def binding_abi() -> str:
+    """The interpreter and torch whose C++ interfaces the binding is compiled against."""
+    import torch
+
+    return (f"{sysconfig.get_config_var('SOABI')} torch {torch.__version__} "
+            f"cxx11abi {int(torch._C._GLIBCXX_USE_CXX11_ABI)}")
+
+
 def binding_needs_build() -> bool:
-    if not BINDING.exists():
+    if not BINDING.exists() or not BINDING_ABI.exists() or BINDING_ABI.read_text() != binding_abi():
         return True
     t = BINDING.stat().st_mtime
     return any(p.stat().st_mtime > t for p in (CSRC / "zs_paged_py.cpp", INCLUDE / "zs.h"))
@@ -64,7 +74,7 @@ def build_binding(force: bool = False, verbose: bool = False) -> Path:
     t = Path(torch.__file__).resolve().parent
     cuda = Path(_nvcc()).resolve().parent.parent
     tmp = BINDING.with_suffix(".so.tmp")
-    cmd = [cxx, "-O2", "-std=c++17", "-shared", "-fPIC",
+    cmd = [cxx, "-O2", "-std=c++17", "-shared", "-fPIC", f'-DZS_BINDING_ABI="{binding_abi()}"',
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", str(INCLUDE),
            "-I", sysconfig.get_paths()["include"], "-I", str(t / "include"),
            "-I", str(t / "include" / "torch" / "csrc" / "api" / "include"), "-I", str(cuda / "include"),
@@ -73,7 +83,9 @@ def build_binding(force: bool = False, verbose: bool = False) -> Path:
     if verbose:
         print(" ".join(cmd))
     subprocess.run(cmd, check=True)
+    BINDING_ABI.unlink(missing_ok=True)   # no moment at which it speaks of another binary
     os.replace(tmp, BINDING)
+    BINDING_ABI.write_text(binding_abi())
     return BINDING
 
 

@@ -27,6 +27,7 @@ import ctypes
 import torch
 
 from . import _lib as Z
+from .build import binding_abi
 
 PAGE_SIZES = (16, 32, 64, 128)
 _DTYPES = (torch.bfloat16, torch.float16)
@@ -44,6 +45,9 @@ def _binding():
         except ImportError as e:
             raise Z.ZsError(f"the paged operators' binding cannot be loaded ({e}): build it with "
                             "__graft_entry__.build()") from e
+        if _paged.abi != binding_abi():
+            _fail(f"the paged operators' binding was built for another Python or torch ({_paged.abi}, not "
+                  f"{binding_abi()}): build it with __graft_entry__.build()")
         _BINDING = _paged
     return _BINDING
 
