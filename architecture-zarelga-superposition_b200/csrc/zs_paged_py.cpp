@@ -68,7 +68,7 @@ double real(PyObject* o, const char* name) {
 void* ptr(const at::Tensor* t) { return t == nullptr ? nullptr : t->data_ptr(); }
 bool misaligned(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 != 0; }
 
-// All on the device of the first, none asking for a gradient.
+// All on the device of the first, none asking for a gradient or carrying a tangent.
 struct Inputs {
   c10::Device device;
   bool grad;
@@ -79,6 +79,8 @@ struct Inputs {
   void look(const at::Tensor& t) const {
     if (grad && t.requires_grad())
       refuse("the paged operators have no gradient: call them under torch.no_grad() or on detached tensors");
+    if (t._fw_grad(0).defined())
+      refuse("the paged operators have no derivative: a tensor carries a forward-mode tangent, which would be lost");
   }
   void add(const at::Tensor* t) const {
     if (t == nullptr) return;
