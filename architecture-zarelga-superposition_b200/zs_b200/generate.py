@@ -8,6 +8,7 @@ since the launches would cost more than the work.
 from __future__ import annotations
 
 import itertools
+import math
 import operator
 
 import torch
@@ -94,10 +95,18 @@ class DecodeStep:
 
 def sample(logits, temperature=0.0, generator=None):
     """Token ids [n]: the largest logit (the lowest id of equals), or with a temperature a draw from
-    softmax(logits / temperature)."""
+    softmax(logits / temperature).  A row without a finite largest logit gets any id: torch.multinomial
+    ends the process's GPU context where a probability is no number."""
+    if math.isnan(temperature):
+        raise Z.ZsError(f"temperature must be a number (got {temperature})")
     if temperature <= 0.0:
         return logits.argmax(-1)
-    p = torch.softmax(logits.float() / temperature, -1)
+    x = logits.float()
+    # the quotients stay numbers at both ends of f32: of the distance to the largest logit, which is zero for
+    # itself, under a small temperature; of the logits, which are finite or -inf, under a large one
+    x = (x - x.amax(-1, keepdim=True)) / max(temperature, 1e-38) if temperature < 1e-3 else x / min(temperature, 1e38)
+    p = torch.softmax(x, -1)
+    p = p.masked_fill(p.isnan(), 1.0)
     return torch.multinomial(p, 1, generator=generator).squeeze(-1)
 
 
