@@ -17,6 +17,19 @@ from . import _lib as Z
 from .dense import one_group_routing
 
 
+def sharded(model):
+    """Whether the model's experts are sharded over ranks."""
+    from scattermoe.expert_parallel import ExpertParallelGLUMLP
+
+    return any(isinstance(m, ExpertParallelGLUMLP) for m in model.modules())
+
+
+def _refuse_sharded(model):
+    if sharded(model):
+        raise Z.ZsError("a decode step cannot be recorded with experts sharded over ranks (their exchange reads its "
+                        "sizes on the host): call forward_paged for every step, on all ranks alike")
+
+
 class DecodeStep:
     """One decode step of all slots of a cache as a CUDA graph: the slots grow by `active` (0 or 1)
     tokens, `tokens` go in, `logits` come out.  A slot that does not grow (inactive, or refused for want
@@ -26,9 +39,11 @@ class DecodeStep:
     recording.  The package's optimizer writes those in place; after any other change (of a weight by a
     torch operation or load_state_dict; another tensor, parameter, buffer or module in the place of one;
     another `model`, `cache`, `slots`, `active` or `tokens`) the step is recorded again.  Changes that no
-    tensor or module shows (a flag, a hook) need `graph = None`."""
+    tensor or module shows (a flag, a hook) need `graph = None`.  Experts sharded over ranks
+    (shard_experts) are refused."""
 
     def __init__(self, model, cache):
+        _refuse_sharded(model)
         dev = cache.kv.device
         n = cache.seq_lens.numel()
         self.model, self.cache = model, cache
@@ -78,6 +93,7 @@ class DecodeStep:
             self.graph.replay()
             self.logits = self._static
             return self.logits
+        _refuse_sharded(self.model)
         # a step outside the recording first (a real one): it makes or refreshes every lazily
         # made buffer, then the next ones are recorded
         self.logits = self._run()
@@ -113,7 +129,9 @@ def sample(logits, temperature=0.0, generator=None):
 @torch.no_grad()
 def generate(model, prompts, max_new_tokens, *, temperature=0.0, eos_token_id=None, page_size=64, generator=None):
     """Continuations (a list of lists of ids) of prompts (a list of non-empty id sequences).  Greedy
-    by default; a sequence ends after eos_token_id (which is part of it) or max_new_tokens ids."""
+    by default; a sequence ends after eos_token_id (which is part of it) or max_new_tokens ids.  Refuses a
+    model whose experts are sharded over ranks (see DecodeStep)."""
+    _refuse_sharded(model)
     prompts = [torch.as_tensor(p, dtype=torch.long).reshape(-1).cpu() for p in prompts]
     if not prompts or min(p.numel() for p in prompts) < 1:
         raise Z.ZsError("generate needs prompts of at least one token")

@@ -145,6 +145,11 @@ class MoELM(nn.Module):
         from .dense import dense_linear
 
         if ids.numel() == 0 and (cu_seqlens is not None or block_table.size(0) == 0):
+            from .generate import sharded
+
+            if sharded(self):
+                raise Z.ZsError("with experts sharded over ranks every rank needs a token (the others wait for its "
+                                "part of the exchange)")
             head = self.output_layer.weight
             return torch.zeros(block_table.size(0), head.size(0), dtype=torch.bfloat16, device=head.device)
         with torch.autocast("cuda", dtype=torch.bfloat16, cache_enabled=False):

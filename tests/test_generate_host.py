@@ -1,6 +1,7 @@
 """The host side of generation: drawing ids (torch refuses a bad probability on the CPU; on a GPU it would end
-the process's context)."""
+the process's context), and models that no step can be recorded for."""
 import math
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -40,3 +41,33 @@ def test_rows_without_a_largest_logit_get_some_id(row):
 def test_a_temperature_that_is_no_number_is_refused():
     with pytest.raises(ZsError, match="temperature"):
         sample(torch.zeros(1, 4), math.nan)
+
+
+def test_sharded_experts_are_refused(tmp_path):
+    import torch.distributed as dist
+
+    from modeling.model_config import ModelConfig
+    from scattermoe.expert_parallel import shard_experts
+    from zs_b200.generate import DecodeStep, generate
+    from zs_b200.lm import MoELM
+
+    cfg = ModelConfig(vocab_size=64, embed_size=128, hidden_size=128, transformer_depth=1, intermediate_size=64,
+                      n_experts=5, n_shared_experts=1, n_attention_heads=2, n_key_value_heads=1,
+                      attention_window_pattern=(None,), max_position_embeddings=64, sequence_length=64)
+    m = MoELM(cfg)
+    cache = SimpleNamespace(kv=torch.zeros(1), seq_lens=torch.zeros(2, dtype=torch.int32))
+    step = DecodeStep(m, cache)
+    dist.init_process_group("gloo", init_method=f"file://{tmp_path}/group", rank=0, world_size=1)
+    try:
+        assert shard_experts(m)
+        with pytest.raises(ZsError, match="sharded"):
+            DecodeStep(m, cache)
+        with pytest.raises(ZsError, match="sharded"):
+            step()                                           # sharded after the step was made
+        with pytest.raises(ZsError, match="sharded"):
+            generate(m, [[1, 2]], 4)
+        none = torch.zeros(2, dtype=torch.int32)
+        with pytest.raises(ZsError, match="every rank"):     # the other ranks would wait for this one
+            m.forward_paged(torch.zeros(0, dtype=torch.long), cache, none.view(1, 2), none[:1], none)
+    finally:
+        dist.destroy_process_group()
