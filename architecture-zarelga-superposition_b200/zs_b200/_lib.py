@@ -194,13 +194,15 @@ def require_cuda(*tensors) -> None:
 
 def device_error(device=None) -> int:
     out = ctypes.c_int(0)
-    check(lib().zs_device_error_get(ctypes.byref(out), torch.cuda.current_stream(device).cuda_stream),
-          "zs_device_error_get")
+    with torch.cuda.device(device):      # each device has a word of its own, found through the current device
+        check(lib().zs_device_error_get(ctypes.byref(out), torch.cuda.current_stream(device).cuda_stream),
+              "zs_device_error_get")
     return out.value
 
 
 def clear_device_error(device=None) -> None:
-    check(lib().zs_device_error_clear(torch.cuda.current_stream(device).cuda_stream), "zs_device_error_clear")
+    with torch.cuda.device(device):
+        check(lib().zs_device_error_clear(torch.cuda.current_stream(device).cuda_stream), "zs_device_error_clear")
 
 
 # ------------------------------------------------------------ instrumentation
