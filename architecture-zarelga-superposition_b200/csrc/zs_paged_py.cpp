@@ -308,13 +308,19 @@ PyObject* attention(PyObject* const* a) {
   return r;
 }
 
-// pages(op, cache, kv, a, b): op 0 extend, 1 fork, 2 free, 3 compact, 4 copy; cache: the address of the zs_kv_cache of
-// the pool kv; a, b: its request lists (None where the operation has none)
+// pages(op, cache, kv, block_table, seq_lens, ref_count, a, b): op 0 extend, 1 fork, 2 free, 3 compact, 4 copy; cache: the
+// address of the zs_kv_cache, which holds the addresses of the four tensors; a, b: its request lists (None where the
+// operation has none)
 PyObject* pages(PyObject* const* a) {
   const long long op = whole(a[0], "op");
   const auto* cache = reinterpret_cast<const zs_kv_cache*>((uintptr_t)whole(a[1], "cache"));
   const at::Tensor& kv = tensor(a[2], "kv");
-  const at::Tensor* lists[2] = {maybe(a[3], "requests"), maybe(a[4], "requests")};
+  const void* held[4] = {cache->kv, cache->block_table, cache->seq_lens, cache->ref_count};
+  for (int i = 0; i < 4; ++i)
+    if (tensor(a[2 + i], "the cache's tensors").data_ptr() != held[i])
+      refuse("the cache's kv, block_table, seq_lens and ref_count stay where it made them: write into them (copy_) "
+             "instead of replacing them");
+  const at::Tensor* lists[2] = {maybe(a[6], "requests"), maybe(a[7], "requests")};
   int64_t n = 0;
   for (const at::Tensor* t : lists) {
     if (t == nullptr) continue;
@@ -367,7 +373,7 @@ PyObject* call(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyMethodDef methods[] = {
     {"append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&call<append, 12>)), METH_FASTCALL, nullptr},
     {"attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&call<attention, 11>)), METH_FASTCALL, nullptr},
-    {"pages", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&call<pages, 5>)), METH_FASTCALL, nullptr},
+    {"pages", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&call<pages, 8>)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_paged", "Paged key-value cache operators (see paged.py).", -1, methods,

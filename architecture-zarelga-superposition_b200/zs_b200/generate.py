@@ -69,7 +69,8 @@ class DecodeStep:
         return t.data_ptr(), None if sh is None else (sh.data_ptr(), t._version)
 
     def _own(self):
-        return self.model, self.cache, self.slots, self.active, self.tokens
+        c = self.cache
+        return self.model, c, c.kv, c.block_table, c.seq_lens, self.slots, self.active, self.tokens
 
     def _remember(self):
         """What the recorded kernels depend on: this object's inputs and every module's modules, parameters and

@@ -103,7 +103,8 @@ class PagedKVCache:
     kv [n_layers, 2, num_pages, n_kv_heads, page_size, head_dim] (keys, values); a slot is a row of
     block_table [max_seqs, max_pages_per_seq] (-1: no page) with its length in seq_lens;
     ref_count [num_pages] counts the rows that hold a page.  The three tables are views of one
-    int32 tensor `meta`, so a copy of it is a snapshot of the bookkeeping.
+    int32 tensor `meta`, so a copy of it is a snapshot of the bookkeeping.  The tensors may be written but
+    not replaced.
 
     Requests are int32 CUDA tensors (a list or int is uploaded); they are served in order and take
     the lowest-numbered free pages.  Nothing here waits for the host: a request that cannot be
@@ -167,7 +168,8 @@ class PagedKVCache:
         if y is not None:
             y = self._list(y)
         Z.INSTR.launches += launches
-        (_BINDING or _binding()).pages(op, ctypes.addressof(self._c), self.kv, x, y)
+        (_BINDING or _binding()).pages(op, ctypes.addressof(self._c), self.kv, self.block_table, self.seq_lens,
+                                       self.ref_count, x, y)
 
     def extend(self, slots, n_tokens):
         """Slot slots[i] grows by n_tokens[i] >= 0 tokens, with pages for them; what they hold is

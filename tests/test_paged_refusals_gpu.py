@@ -1,4 +1,5 @@
-"""Inputs that carry a tangent: the paged operators have no derivative in either direction."""
+"""What the paged operators refuse beside wrong types and sizes: inputs that carry a tangent (they have no derivative
+in either direction), and a cache whose tensors were replaced (its bookkeeping would go on in the old memory)."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
@@ -35,3 +36,23 @@ def test_tangents_are_refused(which):
             x = torch.randn(2, 6 * 64, device="cuda").bfloat16()
             with pytest.raises(ZsError, match="derivative|gradient"):
                 paged.paged_append(x, w["k"], w["v"], w["table"], w["lens"], n_heads=2)
+
+
+@pytest.mark.parametrize("name", ["kv", "block_table", "seq_lens", "ref_count"])
+@pytest.mark.parametrize("how", ["replaced", "moved"])
+def test_a_cache_whose_tensors_were_replaced_is_refused(name, how):
+    from zs_b200 import ZsError, paged
+
+    c = paged.PagedKVCache(1, 1, 64, num_pages=8, page_size=16, max_seqs=2, max_pages_per_seq=4)
+    c.extend([0], [20])
+    old = getattr(c, name)
+    was = old.clone()
+    if how == "replaced":
+        setattr(c, name, old.clone())
+    else:
+        old.data = old.data.clone()
+    for call in (lambda: c.extend([0], [1]), lambda: c.fork([0], [1]), lambda: c.free([0]), lambda: c.compact(),
+                 lambda: c.copy_pages([0], [5])):
+        with pytest.raises(ZsError, match="instead of replacing"):
+            call()
+    assert torch.equal(getattr(c, name), was)
