@@ -70,3 +70,33 @@ def test_a_default_cache_forks_between_full_slots():
         was = [was[1], was[2], was[0]]
         for s in range(3):
             assert torch.equal(held(s), was[s])
+
+
+def test_packed_prompts_through_sparse_routing():
+    """Two of eight experts a token.  A rounding may swap two experts of nearly one score, so sequences are compared
+    whose routing is the same in both paths; short ones, so that most are."""
+    from test_decode_step_gpu import _sparse_model
+
+    cfg, m = _sparse_model()
+    g = torch.Generator().manual_seed(7)
+    seqs = [torch.randint(0, cfg.vocab_size, (1 + i % 6,), generator=g).cuda() for i in range(60)]
+    n = torch.tensor([s.numel() for s in seqs], dtype=torch.int32, device="cuda")
+    cu = torch.cat([n.new_zeros(1), n.cumsum(0).int()])
+    c = m.new_cache(len(seqs), 32, page_size=16)
+    chosen = []
+    hooks = [b.mlp.register_forward_hook(lambda _m, _a, out: chosen.append(out[1][0].sort(-1)[0])) for b in m.layers]
+    c.extend(torch.arange(len(seqs), dtype=torch.int32, device="cuda"), n)
+    got = m.forward_paged(torch.cat(seqs), c, c.block_table, c.seq_lens, cu)
+    for h in hooks:
+        h.remove()
+    assert len(torch.stack(chosen).unique()) == 8            # every expert has tokens
+    alike = 0
+    for i, s in enumerate(seqs):
+        with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16):
+            want, routing = m(s.view(1, -1))
+        rows = slice(int(cu[i]), int(cu[i + 1]))
+        if all(torch.equal(a[rows], b[0].sort(-1)[0]) for a, b in zip(chosen, routing)):
+            alike += 1
+            assert rel_err(got[i], want[0, -1].float()) < TOL
+    assert alike >= len(seqs) // 2
+    c.check()
