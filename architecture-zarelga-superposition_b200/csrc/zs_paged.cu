@@ -91,12 +91,13 @@ struct AppendArgs {
 // A warp holds 256 / hd head rows at a time; a lane has four columns of a row's
 // first half and the same four of its second half (8-byte accesses, whole
 // sectors), so it owns both members of the pairs that rotate.  A warp owns one
-// of `parts` shares of a token's rows.  HBM-bound (each projected value is read
-// once and written once), so what matters is loads in flight: the first rows
-// are asked for before the token's sequence and page are looked up, and cos and
+// of `parts` shares of a token's rows.  Each projected value is read once and
+// written once, and what bounds that is loads in flight and issue slots: the first
+// rows are asked for before the token's sequence and page are looked up, and cos and
 // sin are read once per token.  21K prompt tokens of 16 + 2 * 4 heads of 128: 51 us,
-// 4.9 TB/s (75 % of a copy; about half of the issue slots are used); blocks of four
-// warps, because 28 warps fit an SM then (256 threads, 24 warps: 58 us).
+// 4.9 TB/s in and out (75 % of a copy; DRAM itself is busy 46 % of that time, half of
+// what is written being in L2 still at the end, and 65 % of the issue slots are used);
+// blocks of four warps, because 28 warps fit an SM then (256 threads, 24 warps: 58 us).
 template <typename T>
 __device__ __forceinline__ void unpack4(const uint2& u, float* v) {
   const float2 a = Pair<T>::to_f(*reinterpret_cast<const typename Pair<T>::type*>(&u.x));

@@ -139,9 +139,10 @@ class MoELM(nn.Module):
         """Logits [num_seqs, vocab] after each sequence's last new token.  ids [T]: the packed new
         tokens; cache: a PagedKVCache whose slots already count them (PagedKVCache.extend);
         block_table, seq_lens: the rows of the cache's tables that belong to the sequences;
-        cu_seqlens [num_seqs + 1]: their rows in ids (None: one new token each).  A sequence without new
-        tokens gets a row of zeros; rows behind the last token there is are not read.  Runs under
-        bf16 autocast whatever the caller's context."""
+        cu_seqlens [num_seqs + 1]: their rows in ids (None: one new token each, stored at position
+        seq_lens - 1; a length of 0 stands for a slot without one, whose row means nothing).  With cu_seqlens a
+        sequence without new tokens gets a row of zeros; rows behind the last token there is are not
+        read.  Runs under bf16 autocast whatever the caller's context."""
         from .dense import dense_linear
 
         if ids.numel() == 0 and (cu_seqlens is not None or block_table.size(0) == 0):
