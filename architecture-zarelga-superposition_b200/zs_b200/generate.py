@@ -103,7 +103,9 @@ class DecodeStep:
         with torch.cuda.device(self.tokens.device):
             torch.cuda.current_stream().synchronize()
             graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(graph):
+            # a stream of this device: torch's own one for captures lies on the device of the process's first capture,
+            # and nothing that runs on another device is recorded there
+            with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
                 static = self._run()
         self._remember()
         self.graph, self._static = graph, static

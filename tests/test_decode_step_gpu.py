@@ -175,3 +175,23 @@ def test_a_recorded_step_follows_its_modules_and_buffers(change):
         meta, kv = c.meta.clone(), c.kv.clone()
     assert changed
     c.check()
+
+
+def test_a_step_is_recorded_on_a_stream_of_its_device(monkeypatch):
+    """Not on the stream that torch keeps for captures, which may be another device's."""
+    from zs_b200.generate import DecodeStep
+
+    given, real = [], torch.cuda.graph
+
+    class Graph(real):
+        def __init__(self, graph, **kw):
+            given.append((torch.cuda.current_device(), kw.get("stream")))
+            super().__init__(graph, **kw)
+
+    monkeypatch.setattr(torch.cuda, "graph", Graph)
+    cfg, m = _model(layers=1, windows=(None,))
+    step = DecodeStep(m, m.new_cache(1, 32, page_size=16))
+    step.active.fill_(1)
+    step(), step()
+    ((device, stream),) = given
+    assert stream is not None and stream.device.index == device == step.cache.kv.device.index
