@@ -731,7 +731,8 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const AttnA
 // TMEM columns: S_t / P_t at t * 128, O_t at 256 + t * hd.  P is rounded to the cache's type because the
 // products take 16-bit operands; its sum is taken in f32 before that.
 //
-// One prompt of 32768 tokens, 16/4 heads of 128: 4.05 ms, 1086 TFLOP/s (64 % of a cuBLAS burst).  Bound by
+// One prompt of 32768 tokens, 16/4 heads of 128: 4.01 to 4.16 ms by the clock, 1097 to 1057 TFLOP/s (65 to 62 % of a
+// cuBLAS burst).  Bound by
 // the chain of a query tile: of 3850 cycles for a step of both tiles, softmax takes 2000, products and
 // waits 1700 to 1800, and the two tiles overlap each other's; pure products would take 2100.
 
